@@ -436,6 +436,79 @@ int ptb_gemm_status(int *status, int reset);
  * give-up path and its reporting without provoking a fault.  No counterpart in the reference. */
 int ptb_gemm_wait_selftest(ptb_stream_t stream);
 
+/* ------------------------------------------------------------------ routing ------------------ */
+/* The k experts of every token and their probabilities, from logits [T, E] (PTB_F32 / PTB_F16 / PTB_BF16, row_stride elements
+ * apart).  score_function: PTB_SCORE_SOFTMAX or PTB_SCORE_SIGMOID of the logits; what is compared is the score, plus
+ * bias[e] where bias is not NULL; with groups > 1 only the experts of the topk_groups groups (of E / groups neighbouring experts)
+ * whose two largest add up to most.  Ties go to the lowest index.  A logit of -inf makes an expert unavailable; where fewer than k
+ * are left, the last ids are -1 with probability 0.  NaN counts as the largest.
+ *   probability = scaling * score, or with normalize: scaling * (softmax of the chosen logits; score / (sum of the chosen + 1e-20))
+ * ids [T, k] int64 in falling order of what was compared.  probs [T, k] fp32, or table [T, E] fp32 (0 where not chosen) and map
+ * [T, E] bytes (1 where chosen), or both forms.  E <= 1024, k <= 32, groups <= 32.  table, map: 16-byte aligned.
+ * Fills the place of primus_turbo/pytorch/ops/moe/fused_moe_router.py and the tables that permutation.py takes. */
+#define PTB_SCORE_SOFTMAX 0
+#define PTB_SCORE_SIGMOID 1
+int ptb_topk_router(const void *logits, int dtype, int64_t T, int64_t E, int64_t row_stride, int64_t k,
+                    int score_function, const float *bias, int64_t groups, int64_t topk_groups, int normalize,
+                    float scaling, int64_t *ids, float *probs, float *table, void *map, ptb_stream_t stream);
+
+/* Gradient of ptb_topk_router's probabilities with respect to the logits: grad [T, k] (dense = 0) or [T, E] (dense = 1,
+ * read at the chosen experts alone), rows grad_stride apart; ids as that call wrote them.  grad_logits [T, E] in the logits' type,
+ * 16-byte aligned, every entry written. */
+int ptb_topk_router_bwd(const void *logits, int dtype, int64_t T, int64_t E, int64_t row_stride, int64_t k,
+                        int score_function, int normalize, float scaling, const int64_t *ids, const float *grad,
+                        int64_t grad_stride, int dense, void *grad_logits, ptb_stream_t stream);
+
+/* ------------------------------------------------------------------ 4-bit weights ------------- */
+/* A 4-bit weight of rows x K values: codes, ceil(K / 128) * 64 bytes a row, and per group of 32, 64 or 128 neighbouring values
+ * of a row a bf16 scale and (optionally) a zero point byte, both [rows, ceil(K / group)].  value = (code - zero) * scale; zero is
+ * 8 where zero is NULL.  In a row's block of 128 values, the 32-bit word t * 4 + q (t, q in 0 .. 3) holds the eight values from 32 q +
+ * 8 t on, value i of them in nibble i / 2 + 4 (i % 2); codes past K are 0.  K a multiple of 8; codes 16-byte aligned.
+ *
+ * Quantise: w [rows, K] contiguous, 16-byte aligned, fp32 / fp16 / bf16.
+ *   zero == NULL: scale = bf16(max |w| / 7), otherwise scale = bf16(max(w, 0) / 15 - min(w, 0) / 15) and
+ *   zero = clamp(rint(-min(w, 0) / scale), 0, 15);  code = clamp(rint(w / scale) + zero, 0, 15).
+ * A group that holds a NaN or an infinity gets the scale NaN; a group of zeros the scale 0.  No counterpart in the reference. */
+int ptb_quant_int4(const void *w, int dtype, int64_t rows, int64_t K, int64_t group, void *codes, void *scale,
+                   void *zero, ptb_stream_t stream);
+/* out [rows, K] = the values, in out_dtype (fp32 / fp16 / bf16), 16-byte aligned. */
+int ptb_dequant_int4(const void *codes, const void *scale, const void *zero, int64_t rows, int64_t K, int64_t group,
+                     void *out, int out_dtype, ptb_stream_t stream);
+/* out[m, n] = sum_k x[m, k] * value[n, k] (+ bias[n]), accumulated in fp32; x [M, K] with rows ldx apart (a multiple of 8
+ * where M > 1, 16-byte aligned), bias [N] and out [M, N] in x's type (bf16 or fp16).  Made for few rows; more are taken 32 at a time,
+ * each time with another read of the weight. */
+int ptb_gemm_int4(const void *x, int dtype, int64_t ldx, int64_t M, int64_t N, int64_t K, const void *codes,
+                  const void *scale, const void *zero, int64_t group, const void *bias, void *out,
+                  ptb_stream_t stream);
+
+/* ------------------------------------------------------------------ MoE layer for a few tokens - */
+/* out[t] = sum_j probs[t, j] * W2[e] (silu(u[:I]) * u[I:]), u = W1[e] x[t], e = ids[t, j], for W1 [E, 2 I, H] (gate rows first)
+ * and W2 [E, H, I].  x [T, H] bf16 or fp16, rows ldx apart; ids [T, k] int64 and probs [T, k] fp32, contiguous; an id outside
+ * [0, E) contributes nothing.  out [T, H] in x's type, contiguous.  Sums are kept in fp32, the activation between the two products
+ * in two bf16 parts; equal inputs give equal bits.
+ * format: x's own type code, PTB_E4M3, PTB_E5M2 or PTB_INT4, the same for both weights.  Data contiguous, 16-byte aligned.
+ *   FP8: scale holds fp32 inverse scales, by granularity: PTB_TENSORWISE one, PTB_ROWWISE [E, rows], PTB_BLOCKWISE
+ *        [E, ceil(rows / 128), ceil(K / 128)].  H and I multiples of 16.
+ *   4-bit: the layout of ptb_quant_int4 for E * rows rows; zero may be NULL; one group size for both.  H, I multiples of 8.
+ * T <= PTB_MOE_FEW_MAX_TOKENS, T * k <= PTB_MOE_FEW_MAX_PAIRS, E <= 1024.  workspace: 16-byte aligned, of
+ * ptb_moe_few_tokens_workspace(T, k, I) bytes (-1: sizes out of range); calls that may overlap need one each.
+ * For more tokens the grouped GEMMs above are the way.  No counterpart in the reference. */
+#define PTB_INT4 5
+#define PTB_MOE_FEW_MAX_TOKENS 128
+#define PTB_MOE_FEW_MAX_PAIRS 1024
+typedef struct {
+    const void *data;
+    const void *scale; /* FP8: fp32; 4-bit: bf16 */
+    const void *zero;  /* 4-bit: bytes, or NULL */
+    int granularity;   /* FP8 */
+    int group;         /* 4-bit */
+} PtbExpertWeight;
+int64_t ptb_moe_few_tokens_workspace(int64_t T, int64_t k, int64_t I);
+int ptb_moe_few_tokens(const void *x, int dtype, int64_t ldx, int64_t T, int64_t H, int64_t I, int64_t E,
+                       const int64_t *ids, const float *probs, int64_t k, int format,
+                       const PtbExpertWeight *gate_up, const PtbExpertWeight *down, void *workspace, void *out,
+                       ptb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,7 +7,7 @@ module raises.  There is no fallback path.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_int, c_int64, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
 from pathlib import Path
 
 import torch
@@ -30,7 +30,7 @@ _DTYPE_CODE = {
     torch.float8_e5m2: PTB_E5M2,
 }
 
-_P, _I, _L = c_void_p, c_int, c_int64
+_P, _I, _L, _F = c_void_p, c_int, c_int64, c_float
 
 # name -> argument types; every function returns int except where noted
 _PROTOS = {
@@ -75,11 +75,17 @@ _PROTOS = {
     "ptb_grouped_gemm_mxfp8": [_P, _I, _L, _P, _L, _P, _I, _P, _P, _I, _L, _P, _L, _L, _L, _L, _I, _P],
     "ptb_grouped_gemm_mxfp8_variable_k": [_P, _I, _L, _P, _L, _P, _I, _L, _P, _L, _P, _I, _P, _L, _L, _L, _L, _I, _P],
     "ptb_gemm_mxfp8": [_P, _I, _L, _P, _L, _P, _I, _L, _P, _L, _P, _I, _L, _L, _L, _L, _I, _P],
+    "ptb_topk_router": [_P, _I, _L, _L, _L, _L, _I, _P, _L, _L, _I, _F, _P, _P, _P, _P, _P],
+    "ptb_topk_router_bwd": [_P, _I, _L, _L, _L, _L, _I, _I, _F, _P, _P, _L, _I, _P, _P],
+    "ptb_quant_int4": [_P, _I, _L, _L, _L, _P, _P, _P, _P],
+    "ptb_dequant_int4": [_P, _P, _P, _L, _L, _L, _P, _I, _P],
+    "ptb_gemm_int4": [_P, _I, _L, _L, _L, _L, _P, _P, _P, _L, _P, _P, _P],
+    "ptb_moe_few_tokens": [_P, _I, _L, _L, _L, _L, _L, _P, _P, _L, _I, _P, _P, _P, _P, _P],
     "ptb_gemm_status": [ctypes.POINTER(c_int), _I],
     "ptb_gemm_wait_selftest": [_P],
 }
 
-EXPORTS = ["ptb_version", "ptb_last_error", "ptb_kernels_enqueued", *_PROTOS.keys()]
+EXPORTS = ["ptb_version", "ptb_last_error", "ptb_kernels_enqueued", "ptb_moe_few_tokens_workspace", *_PROTOS.keys()]
 
 
 def _load() -> ctypes.CDLL:
@@ -95,6 +101,8 @@ def _load() -> ctypes.CDLL:
     lib.ptb_last_error.argtypes = []
     lib.ptb_kernels_enqueued.restype = ctypes.c_int64
     lib.ptb_kernels_enqueued.argtypes = []
+    lib.ptb_moe_few_tokens_workspace.restype = ctypes.c_int64
+    lib.ptb_moe_few_tokens_workspace.argtypes = [_L, _L, _L]
     for name, args in _PROTOS.items():
         fn = getattr(lib, name)
         fn.restype = c_int

@@ -23,7 +23,8 @@ LIB_PATH = OUT_DIR / "libptb_b200.so"
 EXT_PATH = OUT_DIR / "ptb_torch.so"
 EXT_SOURCE = CSRC / "torch_ops.cpp"
 
-SOURCES = ["ptb_quant.cu", "ptb_gemm.cu", "ptb_exchange.cu", "ptb_activation.cu", "ptb_mxfp8.cu"]
+SOURCES = ["ptb_quant.cu", "ptb_gemm.cu", "ptb_exchange.cu", "ptb_activation.cu", "ptb_mxfp8.cu", "ptb_router.cu", "ptb_int4.cu",
+           "ptb_moe_few.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",

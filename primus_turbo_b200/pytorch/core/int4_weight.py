@@ -1,0 +1,102 @@
+"""``Int4Weight``: a weight of 4-bit codes with a scale (and optionally a zero point) per group of a row.
+
+``value[..., n, k] = (code - zero) * scale`` with one bf16 ``scale`` and one byte ``zero`` (8 where there are none) per
+``group_size`` neighbouring ``k`` of a row.  ``qdata`` holds the codes as the kernels read them, ``ceil(K / 128) * 64`` bytes a
+row (the order is described in ``include/ptb.h``); ``from_codes`` and ``codes`` convert from and to one code a byte.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+INT4_GROUP_SIZES = (32, 64, 128)
+INT4_BLOCK = 128  # values per block of the packed layout
+INT4_BLOCK_BYTES = INT4_BLOCK // 2
+
+# byte b of a 32-bit word holds value _LOW[b] of its eight in the low nibble and _HIGH[b] in the high one
+_LOW, _HIGH = (0, 4, 1, 5), (2, 6, 3, 7)
+
+
+def _packed_bytes(k: int) -> int:
+    return (k + INT4_BLOCK - 1) // INT4_BLOCK * INT4_BLOCK_BYTES
+
+
+@dataclass(frozen=True)
+class Int4Weight:
+    """``[N, K]`` or ``[E, N, K]``; made by ``quantize_int4`` or ``from_codes``."""
+
+    qdata: torch.Tensor  # uint8 [..., N, ceil(K / 128) * 64]
+    scale: torch.Tensor  # bfloat16 [..., N, ceil(K / group_size)]
+    zero: Optional[torch.Tensor]  # uint8, like scale
+    shape: torch.Size
+    group_size: int
+
+    def __post_init__(self):
+        object.__setattr__(self, "shape", torch.Size(self.shape))
+        assert self.group_size in INT4_GROUP_SIZES, f"group_size must be one of {INT4_GROUP_SIZES}, got {self.group_size}"
+        assert len(self.shape) in (2, 3), f"a 4-bit weight is 2D or 3D, got {len(self.shape)}D"
+        k = self.shape[-1]
+        assert k % 8 == 0, f"the row length of a 4-bit weight must be a multiple of 8, got {k}"
+        lead = tuple(self.shape[:-1])
+        want = (*lead, _packed_bytes(k))
+        assert self.qdata.dtype == torch.uint8 and tuple(self.qdata.shape) == want, f"qdata must be uint8 {want}"
+        groups = (*lead, (k + self.group_size - 1) // self.group_size)
+        assert self.scale.dtype == torch.bfloat16 and tuple(self.scale.shape) == groups, f"scale must be bfloat16 {groups}"
+        parts = [self.qdata, self.scale]
+        if self.zero is not None:
+            assert self.zero.dtype == torch.uint8 and tuple(self.zero.shape) == groups, f"zero must be uint8 {groups}"
+            parts.append(self.zero)
+        for t in parts:
+            assert t.is_contiguous() and t.device == self.qdata.device, "the parts of a 4-bit weight are contiguous and on one device"
+
+    @property
+    def device(self) -> torch.device:
+        return self.qdata.device
+
+    @property
+    def ndim(self) -> int:
+        return len(self.shape)
+
+    def size(self, dim: int) -> int:
+        return self.shape[dim]
+
+    def to(self, device) -> "Int4Weight":
+        zero = None if self.zero is None else self.zero.to(device)
+        return Int4Weight(self.qdata.to(device), self.scale.to(device), zero, self.shape, self.group_size)
+
+    @classmethod
+    def from_codes(
+        cls, codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor] = None, *, group_size: int
+    ) -> "Int4Weight":
+        """From codes 0 .. 15, one a byte, ``[..., N, K]``; ``scale`` and ``zero`` ``[..., N, ceil(K / group_size)]``."""
+        assert codes.dtype == torch.uint8, "codes must be uint8, one code (0 .. 15) a byte"
+        k = codes.shape[-1]
+        assert k % 8 == 0, f"the row length of a 4-bit weight must be a multiple of 8, got {k}"
+        padded = torch.nn.functional.pad(codes, (0, -k % INT4_BLOCK)) if k % INT4_BLOCK else codes
+        octets = padded.unflatten(-1, (-1, 4, 4, 8)).transpose(-2, -3)  # [..., block, t, q, 8]
+        low, high = (_pick(octets, at) for at in (_LOW, _HIGH))
+        qdata = (low & 15 | high << 4).flatten(-4).contiguous()
+        return cls(qdata, scale.to(torch.bfloat16).contiguous(), None if zero is None else zero.contiguous(), codes.shape, group_size)
+
+    def codes(self) -> torch.Tensor:
+        """The codes, one a byte, ``[..., N, K]``."""
+        words = self.qdata.unflatten(-1, (-1, 4, 4, 4))  # [..., block, t, q, byte]
+        octets = torch.empty((*words.shape[:-1], 8), dtype=torch.uint8, device=self.device)
+        for b in range(4):
+            octets[..., _LOW[b]] = words[..., b] & 15
+            octets[..., _HIGH[b]] = words[..., b] >> 4
+        return octets.transpose(-2, -3).flatten(-4)[..., : self.shape[-1]].contiguous()
+
+    def __repr__(self) -> str:
+        kind = "symmetric" if self.zero is None else "zero points"
+        return f"Int4Weight(shape={tuple(self.shape)}, group_size={self.group_size}, {kind}, device={self.device})"
+
+
+def _pick(octets: torch.Tensor, at) -> torch.Tensor:
+    return torch.stack([octets[..., i] for i in at], dim=-1)
+
+
+__all__ = ["Int4Weight", "INT4_GROUP_SIZES"]

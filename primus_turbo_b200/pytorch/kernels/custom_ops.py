@@ -10,6 +10,7 @@ from typing import List, Optional, Tuple
 
 import torch
 
+from primus_turbo_b200.pytorch.kernels import few_rows_impl as _f
 from primus_turbo_b200.pytorch.kernels import gemm_impl as _g
 from primus_turbo_b200.pytorch.kernels import quantization_impl as _q
 
@@ -182,6 +183,85 @@ def _(a, b, a_scales, b_scales, group_lens, group_offs, trans_a, trans_b, trans_
     return torch.empty((G, m, n), dtype=out_dtype, device=a.device)
 
 
+# ---- routing, 4-bit weights, MoE layer for a few tokens ---------------------------------------------------------
+@torch.library.custom_op(f"{_NS}::topk_router", mutates_args=())
+def topk_router(
+    logits: torch.Tensor, topk: int, score_function: int, expert_bias: Optional[torch.Tensor], num_groups: int, topk_groups: int,
+    normalize: bool, scaling_factor: float, dense: bool,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _f.topk_router_impl(logits, topk, score_function, expert_bias, num_groups, topk_groups, normalize, scaling_factor, dense)
+
+
+@topk_router.register_fake
+def _(logits, topk, score_function, expert_bias, num_groups, topk_groups, normalize, scaling_factor, dense):
+    T, E = logits.shape
+    return (logits.new_empty((T, topk), dtype=torch.int64), logits.new_empty((T, E if dense else topk), dtype=torch.float32),
+            logits.new_empty((T, E) if dense else (0,), dtype=torch.bool))
+
+
+@torch.library.custom_op(f"{_NS}::topk_router_bwd", mutates_args=())
+def topk_router_bwd(
+    logits: torch.Tensor, ids: torch.Tensor, grad: torch.Tensor, score_function: int, normalize: bool, scaling_factor: float, dense: bool
+) -> torch.Tensor:
+    return _f.topk_router_bwd_impl(logits, ids, grad, score_function, normalize, scaling_factor, dense)
+
+
+@topk_router_bwd.register_fake
+def _(logits, ids, grad, score_function, normalize, scaling_factor, dense):
+    return logits.new_empty(logits.shape)
+
+
+@torch.library.custom_op(f"{_NS}::quant_int4", mutates_args=())
+def quant_int4(w: torch.Tensor, group_size: int, symmetric: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _f.quant_int4_impl(w, group_size, symmetric)
+
+
+@quant_int4.register_fake
+def _(w, group_size, symmetric):
+    lead, k = w.shape[:-1], w.shape[-1]
+    groups = (*lead, _cdiv(k, group_size))
+    return (w.new_empty((*lead, _cdiv(k, 128) * 64), dtype=torch.uint8), w.new_empty(groups, dtype=torch.bfloat16),
+            w.new_empty((0,) if symmetric else groups, dtype=torch.uint8))
+
+
+@torch.library.custom_op(f"{_NS}::dequant_int4", mutates_args=())
+def dequant_int4(
+    codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor], k: int, group_size: int, out_dtype: torch.dtype
+) -> torch.Tensor:
+    return _f.dequant_int4_impl(codes, scale, zero, k, group_size, out_dtype)
+
+
+@dequant_int4.register_fake
+def _(codes, scale, zero, k, group_size, out_dtype):
+    return codes.new_empty((*codes.shape[:-1], k), dtype=out_dtype)
+
+
+@torch.library.custom_op(f"{_NS}::gemm_int4", mutates_args=())
+def gemm_int4(
+    x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor], group_size: int, bias: Optional[torch.Tensor]
+) -> torch.Tensor:
+    return _f.gemm_int4_impl(x, codes, scale, zero, group_size, bias)
+
+
+@gemm_int4.register_fake
+def _(x, codes, scale, zero, group_size, bias):
+    return x.new_empty((x.shape[0], codes.shape[0]))
+
+
+@torch.library.custom_op(f"{_NS}::moe_few_tokens", mutates_args=())
+def moe_few_tokens(
+    x: torch.Tensor, ids: torch.Tensor, probs: torch.Tensor, w1: torch.Tensor, w1_scale: Optional[torch.Tensor],
+    w1_zero: Optional[torch.Tensor], w2: torch.Tensor, w2_scale: Optional[torch.Tensor], w2_zero: Optional[torch.Tensor],
+    inter: int, granularity: int, group_size: int,
+) -> torch.Tensor:
+    return _f.moe_few_tokens_impl(x, ids, probs, w1, w1_scale, w1_zero, w2, w2_scale, w2_zero, inter, granularity, group_size)
+
+
+@moe_few_tokens.register_fake
+def _(x, ids, probs, w1, w1_scale, w1_zero, w2, w2_scale, w2_zero, inter, granularity, group_size):
+    return x.new_empty(x.shape)
+
+
 # ---- eager fast path ----------------------------------------------------------------------------------------
 # Outside tracing, a registered op's Python dispatcher (autograd wrapper, redispatch, dynamo frame guard) costs
 # about 70 us per call -- several times the ctypes call it wraps, and with six such calls per grouped-GEMM
@@ -205,6 +285,7 @@ def _with_eager_fast_path(op):
 
 for _name in ("quantize_fp8_tensorwise", "quantize_fp8_rowwise", "quant_fp8_blockwise", "quant_fp8_blockwise_dual",
               "quant_fp8_blockwise_for_weight", "quant_fp8_blockwise_segment_m_row_col", "dequantize_fp8", "gemm_fp8_impl",
-              "grouped_gemm_fp8_impl", "grouped_gemm_fp8_variable_k_impl"):
+              "grouped_gemm_fp8_impl", "grouped_gemm_fp8_variable_k_impl", "topk_router", "topk_router_bwd", "quant_int4",
+              "dequant_int4", "gemm_int4", "moe_few_tokens"):
     globals()[_name] = _with_eager_fast_path(globals()[_name])
 del _name

@@ -1,0 +1,210 @@
+"""4-bit weights against a plain form in 64 bits: codes, scales and zero points equal, products to the accuracy of fp32 sums
+and one rounding.  Every group size and row tail, row counts on both sides of the eights, strides, special values."""
+
+import math
+
+import pytest
+import torch
+
+from primus_turbo_b200.pytorch.core.int4_weight import Int4Weight
+from primus_turbo_b200.pytorch.ops import dequantize_int4, gemm_int4, quantize_int4
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def spread(t, group, k):
+    return t.repeat_interleave(group, dim=-1)[..., :k]
+
+
+def reference_quant(w, group, symmetric):
+    """(codes, scale, zero) of a finite weight, in 64 bits."""
+    k = w.shape[-1]
+    wide = torch.nn.functional.pad(w.double(), (0, -k % group)).unflatten(-1, (-1, group))
+    lo, hi = wide.amin(-1).clamp(max=0), wide.amax(-1).clamp(min=0)
+    scale = ((torch.maximum(hi, -lo) / 7) if symmetric else (hi - lo) / 15).to(torch.bfloat16)
+    s = scale.double()
+    zero = torch.full_like(s, 8) if symmetric else torch.where(s > 0, (-lo / s).round().clamp(0, 15), 0.0)
+    steps = torch.where(s[..., None] > 0, wide / s[..., None], 0.0).round()
+    codes = (steps + zero[..., None]).clamp(0, 15).flatten(-2)[..., :k].to(torch.uint8)
+    return codes, scale, zero.to(torch.uint8)
+
+
+@pytest.mark.parametrize("shape", [(1, 8), (3, 32), (5, 40), (7, 120), (4, 128), (9, 136), (17, 1000), (2, 3, 264), (33, 4096)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_quantise(shape, group, symmetric, dtype):
+    torch.manual_seed(shape[-1] + group)
+    w = (torch.randn(shape, device=DEV) * torch.rand((*shape[:-1], 1), device=DEV)).to(dtype)
+    q = quantize_int4(w, group_size=group, symmetric=symmetric)
+    codes, scale, zero = reference_quant(w, group, symmetric)
+    assert torch.equal(q.scale, scale)
+    if symmetric:
+        assert q.zero is None
+    else:
+        assert torch.equal(q.zero, zero)
+    assert torch.equal(q.codes(), codes)
+    # the stored form is the one that from_codes makes, padding included
+    assert torch.equal(Int4Weight.from_codes(codes, scale, q.zero, group_size=group).qdata, q.qdata)
+    for out in (torch.float32, dtype):
+        z = spread(zero, group, shape[-1]).double()
+        want = ((codes.double() - z) * spread(scale, group, shape[-1]).double()).to(out)
+        assert torch.equal(dequantize_int4(q, out), want)
+
+
+def test_quantise_fp32_is_within_half_a_step():
+    torch.manual_seed(0)
+    w = torch.randn(64, 520, device=DEV)
+    for symmetric in (True, False):
+        q = quantize_int4(w, group_size=64, symmetric=symmetric)
+        s = spread(q.scale, 64, 520).double()
+        # half a step, and what the clamp takes where the scale's rounding (2^-8 of 7 or 15 steps) or the zero point's (half a step) cut the range
+        assert bool(((dequantize_int4(q, torch.float32).double() - w.double()).abs() <= s * (0.5 + (0.03 if symmetric else 0.56))).all())
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+def test_quantise_special_values(symmetric):
+    w = torch.zeros(6, 128, device=DEV, dtype=torch.bfloat16)
+    w[1, 5] = math.nan
+    w[2, 40] = math.inf
+    w[3, 70] = -math.inf
+    w[4, :] = 1e-38  # the scale of its groups is subnormal
+    w[5, 0], w[5, 1] = torch.finfo(torch.bfloat16).max / 2, torch.finfo(torch.bfloat16).min / 2
+    q = quantize_int4(w, group_size=32, symmetric=symmetric)
+    v = dequantize_int4(q, torch.float32)
+    assert not v[0].any() and not v[1, 32:].any() and bool(v[1, :32].isnan().all())
+    assert bool(v[2, 32:64].isnan().all()) and not v[2, :32].any() and bool(v[3, 64:96].isnan().all())
+    assert bool(((v[4] - 1e-38).abs() < 1e-39).all())
+    assert bool(v[5].isfinite().all()) and v[5, 0] > 1.5e38 and v[5, 1] < -1.5e38
+    assert bool((q.codes()[0] == (8 if symmetric else 0)).all())
+
+
+def test_ties_go_to_the_even_code():
+    w = torch.tensor([[7.0, 0.5, 1.5, 2.5, -0.5, -1.5, -2.5, 3.5]], device=DEV, dtype=torch.bfloat16)
+    q = quantize_int4(w, group_size=32)
+    assert q.scale.item() == 1.0 and q.codes().tolist() == [[15, 8, 10, 10, 8, 6, 6, 12]]
+
+
+def weight(shape, group, zeros, seed=0):
+    g = torch.Generator(DEV).manual_seed(seed)
+    k = shape[-1]
+    groups = (*shape[:-1], -(-k // group))
+    codes = torch.randint(0, 16, shape, generator=g, device=DEV, dtype=torch.uint8)
+    scale = (torch.rand(groups, generator=g, device=DEV) + 0.5).to(torch.bfloat16) * k**-0.5
+    zero = torch.randint(0, 16, groups, generator=g, device=DEV, dtype=torch.uint8) if zeros else None
+    return Int4Weight.from_codes(codes, scale, zero, group_size=group)
+
+
+def values(q):
+    k = q.shape[-1]
+    z = 8.0 if q.zero is None else spread(q.zero, q.group_size, k).double()
+    return (q.codes().double() - z) * spread(q.scale, q.group_size, k).double()
+
+
+def assert_product(y, x, q, bias=None):
+    w, xd = values(q), x.double()
+    want, size = xd @ w.T, xd.abs() @ w.abs().T
+    if bias is not None:
+        want, size = want + bias.double(), size + bias.double().abs()
+    # a product passes through the sums of a group (8), of the blocks of a warp (K / 1024 + 1), of the warps and halves (20) and the bias, each
+    # within 2^-23 (the MMA may cut where it does not round) of a partial sum; then one rounding to the output
+    k = x.shape[-1]
+    tol = size * (k / 1024 + 31) * 2.0**-23 + want.abs() * torch.finfo(y.dtype).eps / 2 + torch.finfo(y.dtype).smallest_normal * torch.finfo(y.dtype).eps
+    assert bool(((y.double() - want).abs() <= tol).all()), ((y.double() - want).abs() / tol).max()
+
+
+@pytest.mark.parametrize("m", [1, 2, 7, 8, 9, 16, 17, 31, 32, 33, 64, 65, 100, 130])
+@pytest.mark.parametrize("n,k", [(1, 8), (16, 128), (37, 520), (300, 1152), (129, 2880)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_product(m, n, k, group):
+    dtype = torch.float16 if (m + n) % 2 else torch.bfloat16
+    q = weight((n, k), group, zeros=(m % 3 == 0), seed=m)
+    x = torch.randn(m, k, device=DEV).to(dtype)
+    bias = torch.randn(n, device=DEV).to(dtype) if m % 2 else None
+    assert_product(gemm_int4(x, q, bias), x, q, bias)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 14336), (5, 14336, 4096), (64, 8192, 8192), (24, 5760, 2880), (48, 1000, 14328)])
+def test_product_of_large_weights(m, n, k):
+    q = weight((n, k), 128, zeros=True, seed=k)
+    x = torch.randn(m, k, device=DEV, dtype=torch.bfloat16)
+    assert_product(gemm_int4(x, q), x, q)
+
+
+def test_product_shapes_and_strides():
+    q = weight((48, 264), 64, True)
+    base = torch.randn(40, 400, device=DEV, dtype=torch.bfloat16)
+    for x in (base[:9, :264], base[:9, 8:272], base[:9, 1:265], base[::3, :264], torch.randn(264, 9, device=DEV, dtype=torch.bfloat16).t(),
+              base[:1, :264].expand(5, 264), torch.randn(2, 3, 264, device=DEV, dtype=torch.bfloat16), base[0, :264], base[:0, :264]):
+        y = gemm_int4(x, q)
+        assert y.shape == (*x.shape[:-1], 48) and y.is_contiguous()
+        assert_product(y.reshape(-1, 48), x.reshape(-1, 264), q)
+    # codes that start in the middle of a 16-byte piece
+    raw = torch.empty(q.qdata.numel() + 4, dtype=torch.uint8, device=DEV)
+    part = raw[4:].view(q.qdata.shape)
+    part.copy_(q.qdata)
+    q2 = Int4Weight(part, q.scale, q.zero, q.shape, q.group_size)
+    assert torch.equal(gemm_int4(base[:9, :264], q2), gemm_int4(base[:9, :264], q))
+    assert torch.equal(dequantize_int4(q2), dequantize_int4(q))
+
+
+def test_product_special_values():
+    """A NaN or an infinity stays in its row of x and its row of the weight."""
+    q = weight((40, 256), 64, True)
+    x = torch.randn(11, 256, device=DEV, dtype=torch.bfloat16)
+    want = gemm_int4(x, q)
+    x2 = x.clone()
+    x2[3, 100] = math.nan
+    x2[10, 7] = math.inf
+    y = gemm_int4(x2, q)
+    assert bool(y[3].isnan().all()) and not bool(y[10].isfinite().any())
+    keep = [i for i in range(11) if i not in (3, 10)]
+    assert torch.equal(y[keep], want[keep])
+    scale = q.scale.clone()
+    scale[5, 1] = math.nan
+    y = gemm_int4(x, Int4Weight(q.qdata, scale, q.zero, q.shape, 64))
+    assert bool(y[:, 5].isnan().all()) and torch.equal(y[:, [i for i in range(40) if i != 5]], want[:, [i for i in range(40) if i != 5]])
+
+
+def test_product_is_repeatable_and_captured():
+    q = weight((2048, 4096), 128, False)
+    x = torch.randn(8, 4096, device=DEV, dtype=torch.bfloat16)
+    y = gemm_int4(x, q)
+    assert torch.equal(y, gemm_int4(x, q))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        z = gemm_int4(x, q)
+        d = dequantize_int4(q)
+        r = quantize_int4(d)
+    x.copy_(torch.randn_like(x))
+    graph.replay()
+    assert torch.equal(z, gemm_int4(x, q)) and torch.equal(d, dequantize_int4(q)) and torch.equal(r.qdata, quantize_int4(d).qdata)
+
+
+def test_a_weight_is_ready_for_the_product_that_follows():
+    """Quantise and multiply in a row, without a wait between: the product reads what the quantiser wrote."""
+    x = torch.randn(4, 512, device=DEV, dtype=torch.bfloat16)
+    for seed in range(20):
+        w = torch.randn(256, 512, device=DEV, dtype=torch.bfloat16, generator=torch.Generator(DEV).manual_seed(seed))
+        y = gemm_int4(x, quantize_int4(w, 64))
+        q = quantize_int4(w, 64)
+        torch.cuda.synchronize()
+        assert torch.equal(y, gemm_int4(x, q))
+
+
+def test_offsets_past_32_bits():
+    n, k = 70000, 65536  # 2.3 GB of codes, 4.6 G values
+    q = quantize_int4(torch.zeros(1, k, device=DEV, dtype=torch.bfloat16), 128)
+    codes = q.qdata.repeat(n, 1)
+    scale = torch.full((n, k // 128), 1.0, device=DEV, dtype=torch.bfloat16)
+    codes[-1, 0] = 0x98  # the last row's value 0 is 0, value 2 is one
+    big = Int4Weight(codes, scale, None, torch.Size((n, k)), 128)
+    x = torch.zeros(1, k, device=DEV, dtype=torch.bfloat16)
+    x[0, 2] = 3.0
+    y = gemm_int4(x, big)
+    assert y[0, -1] == 3.0 and not y[0, :-1].any()
+    v = dequantize_int4(big)
+    assert v[-1, 2] == 1.0 and v[-1].sum() == 1.0
+    again = quantize_int4(v, 128)
+    assert torch.equal(again.codes()[-1, :4].cpu(), torch.tensor([8, 8, 15, 8], dtype=torch.uint8)) and bool((again.qdata[:-1] == 0x88).all())

@@ -424,7 +424,8 @@ int ptb_grouped_gemm_fp8_variable_k(const void *lhs, int lhs_dtype, int64_t ld_l
                                     ptb_stream_t stream);
 
 /* Every device-side wait in the GEMM kernels is bounded (2 s); a kernel whose wait runs out
- * records a non-zero code (1 copy producer, 2 MMA issuer, 3 epilogue, 4 scale loader) and
+ * records a non-zero code (1 copy producer, 2 MMA issuer, 3 epilogue, 4 scale loader, 5 a weight copy of the 4-bit
+ * product or the MoE layer for few tokens) and
  * leaves normally.  This call copies that code to *status (a host pointer) and optionally
  * clears it.  It synchronises with the device.  The code is one word per GPU, shared by every
  * stream and caller of the library in the process: a non-zero value says that some GEMM launched
@@ -463,7 +464,7 @@ int ptb_topk_router_bwd(const void *logits, int dtype, int64_t T, int64_t E, int
 /* A 4-bit weight of rows x K values: codes, ceil(K / 128) * 64 bytes a row, and per group of 32, 64 or 128 neighbouring values
  * of a row a bf16 scale and (optionally) a zero point byte, both [rows, ceil(K / group)].  value = (code - zero) * scale; zero is
  * 8 where zero is NULL.  In a row's block of 128 values, the 32-bit word t * 4 + q (t, q in 0 .. 3) holds the eight values from 32 q +
- * 8 t on, value i of them in nibble i / 2 + 4 (i % 2); codes past K are 0.  K a multiple of 8; codes 16-byte aligned.
+ * 8 t on: value i of them in bits 8 (i % 4) + 4 (i / 4) on.  Codes past K are 0.  K a multiple of 8; codes 16-byte aligned.
  *
  * Quantise: w [rows, K] contiguous, 16-byte aligned, fp32 / fp16 / bf16.
  *   zero == NULL: scale = bf16(max |w| / 7), otherwise scale = bf16(max(w, 0) / 15 - min(w, 0) / 15) and
@@ -476,9 +477,11 @@ int ptb_dequant_int4(const void *codes, const void *scale, const void *zero, int
                      void *out, int out_dtype, ptb_stream_t stream);
 /* out[m, n] = sum_k x[m, k] * value[n, k] (+ bias[n]), accumulated in fp32; x [M, K] with rows ldx apart (a multiple of 8
  * where M > 1, 16-byte aligned), bias [N] and out [M, N] in x's type (bf16 or fp16).  Made for few rows; more are taken 32 at a time,
- * each time with another read of the weight. */
+ * each time with another read of the weight.  workspace: 16-byte aligned, of ptb_gemm_int4_workspace bytes.  A row of x that holds a NaN or
+ * an infinity gives NaN. */
+int64_t ptb_gemm_int4_workspace(int dtype, int64_t M, int64_t K, int64_t group);
 int ptb_gemm_int4(const void *x, int dtype, int64_t ldx, int64_t M, int64_t N, int64_t K, const void *codes,
-                  const void *scale, const void *zero, int64_t group, const void *bias, void *out,
+                  const void *scale, const void *zero, int64_t group, const void *bias, void *workspace, void *out,
                   ptb_stream_t stream);
 
 /* ------------------------------------------------------------------ MoE layer for a few tokens - */
@@ -491,7 +494,7 @@ int ptb_gemm_int4(const void *x, int dtype, int64_t ldx, int64_t M, int64_t N, i
  *        [E, ceil(rows / 128), ceil(K / 128)].  H and I multiples of 16.
  *   4-bit: the layout of ptb_quant_int4 for E * rows rows; zero may be NULL; one group size for both.  H, I multiples of 8.
  * T <= PTB_MOE_FEW_MAX_TOKENS, T * k <= PTB_MOE_FEW_MAX_PAIRS, E <= 1024.  workspace: 16-byte aligned, of
- * ptb_moe_few_tokens_workspace(T, k, I) bytes (-1: sizes out of range); calls that may overlap need one each.
+ * ptb_moe_few_tokens_workspace bytes (-1: sizes out of range); calls that may overlap need one each.
  * For more tokens the grouped GEMMs above are the way.  No counterpart in the reference. */
 #define PTB_INT4 5
 #define PTB_MOE_FEW_MAX_TOKENS 128
@@ -503,7 +506,7 @@ typedef struct {
     int granularity;   /* FP8 */
     int group;         /* 4-bit */
 } PtbExpertWeight;
-int64_t ptb_moe_few_tokens_workspace(int64_t T, int64_t k, int64_t I);
+int64_t ptb_moe_few_tokens_workspace(int dtype, int64_t T, int64_t H, int64_t I, int64_t k, int format);
 int ptb_moe_few_tokens(const void *x, int dtype, int64_t ldx, int64_t T, int64_t H, int64_t I, int64_t E,
                        const int64_t *ids, const float *probs, int64_t k, int format,
                        const PtbExpertWeight *gate_up, const PtbExpertWeight *down, void *workspace, void *out,

@@ -79,13 +79,14 @@ _PROTOS = {
     "ptb_topk_router_bwd": [_P, _I, _L, _L, _L, _L, _I, _I, _F, _P, _P, _L, _I, _P, _P],
     "ptb_quant_int4": [_P, _I, _L, _L, _L, _P, _P, _P, _P],
     "ptb_dequant_int4": [_P, _P, _P, _L, _L, _L, _P, _I, _P],
-    "ptb_gemm_int4": [_P, _I, _L, _L, _L, _L, _P, _P, _P, _L, _P, _P, _P],
+    "ptb_gemm_int4": [_P, _I, _L, _L, _L, _L, _P, _P, _P, _L, _P, _P, _P, _P],
     "ptb_moe_few_tokens": [_P, _I, _L, _L, _L, _L, _L, _P, _P, _L, _I, _P, _P, _P, _P, _P],
     "ptb_gemm_status": [ctypes.POINTER(c_int), _I],
     "ptb_gemm_wait_selftest": [_P],
 }
 
-EXPORTS = ["ptb_version", "ptb_last_error", "ptb_kernels_enqueued", "ptb_moe_few_tokens_workspace", *_PROTOS.keys()]
+EXPORTS = ["ptb_version", "ptb_last_error", "ptb_kernels_enqueued", "ptb_moe_few_tokens_workspace",
+           "ptb_gemm_int4_workspace", *_PROTOS.keys()]
 
 
 def _load() -> ctypes.CDLL:
@@ -102,7 +103,9 @@ def _load() -> ctypes.CDLL:
     lib.ptb_kernels_enqueued.restype = ctypes.c_int64
     lib.ptb_kernels_enqueued.argtypes = []
     lib.ptb_moe_few_tokens_workspace.restype = ctypes.c_int64
-    lib.ptb_moe_few_tokens_workspace.argtypes = [_L, _L, _L]
+    lib.ptb_moe_few_tokens_workspace.argtypes = [_I, _L, _L, _L, _L, _I]
+    lib.ptb_gemm_int4_workspace.restype = ctypes.c_int64
+    lib.ptb_gemm_int4_workspace.argtypes = [_I, _L, _L, _L]
     for name, args in _PROTOS.items():
         fn = getattr(lib, name)
         fn.restype = c_int

@@ -43,6 +43,10 @@ inline int cuda_fail(cudaError_t e, const char *where) {
         if (_e != cudaSuccess) return ::ptb::cuda_fail(_e, #expr);    \
     } while (0)
 
+// the status words of ptb_int4.cu's and ptb_moe_few.cu's kernels, read (and cleared) by ptb_gemm_status
+int int4_status(int *status, int reset);
+int moe_few_status(int *status, int reset);
+
 void count_kernel(); // one more kernel enqueued by this process (ptb_kernels_enqueued)
 
 // after every kernel launch, once

@@ -1318,7 +1318,8 @@ int ptb_gemm_status(int *status, int reset) {
         int zero = 0;
         PTB_CUDA(cudaMemcpyToSymbol(g_gemm_status, &zero, sizeof(int)));
     }
-    return 0;
+    if (int rc = int4_status(status, reset)) return rc;
+    return moe_few_status(status, reset);
 }
 
 int ptb_gemm_fp8(const void *a, int a_dtype, int trans_a, int64_t lda, const void *b, int b_dtype, int trans_b,

@@ -1,5 +1,5 @@
 // 4-bit weights: quantise, dequantise, and the product of a few rows with one.  The layout is described in ptb_few_rows.cuh.
-#include "ptb_few_rows.cuh"
+#include "ptb_few_tokens.cuh"
 
 namespace ptb {
 namespace {
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(256) int4_quant_kernel(const T *w, int64_t oct
         for (int j = 0; j < 8; ++j) {
             const float steps = plain ? code_steps(v[j], s, inv) : rintf(fminf(fmaxf(__fdiv_rn(v[j], s), -16.0f), 16.0f));
             const int c       = min(max((int) steps + z, 0), 15);
-            word |= (uint32_t) c << ((j / 2 + (j & 1) * 4) * 4);
+            word |= (uint32_t) c << int4_shift(j);
         }
     } else {
         word = 0x11111111u * (uint32_t) z;
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(256) int4_dequant_kernel(const uint32_t *codes
     const uint32_t word = codes[(row * (octets_per_row / 16) + o / 16) * 16 + (o & 3) * 4 + ((o >> 2) & 3)];
     T r[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r[j] = from_f32<T>((float) ((int) (word >> ((j / 2 + (j & 1) * 4) * 4) & 15) - z) * s);
+    for (int j = 0; j < 8; ++j) r[j] = from_f32<T>((float) ((int) (word >> int4_shift(j) & 15) - z) * s);
     uint4 u[sizeof(T) / 2];
     memcpy(u, r, sizeof(r));
     uint4 *p = reinterpret_cast<uint4 *>(out + row * K + k);
@@ -125,7 +125,8 @@ __global__ void __launch_bounds__(256) int4_dequant_kernel(const uint32_t *codes
 // ---- product of a few rows ----------------------------------------------------------------------------------------------
 struct Int4GemmArgs {
     const void *x;
-    int64_t ldx; // elements
+    int64_t ldx;
+    ScaledRows xs;
     int M, N, K;
     const uint8_t *codes;
     const __nv_bfloat16 *scale;
@@ -134,84 +135,113 @@ struct Int4GemmArgs {
     void *out;
 };
 
-constexpr int kGemmWarps = 8;
+template <int G> struct Int4Rows { // a lane's two rows of the weight
+    const uint8_t *row[2];
+    RowScale<kWInt4> scale[2];
+    __device__ __forceinline__ void aim(const Int4GemmArgs &a, int n0) {
+        const int blocks = (a.K + kKB - 1) / kKB, groups = (a.K + G - 1) / G;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t r = min(n0 + (((int) threadIdx.x & 31) >> 2) + 8 * h, a.N - 1);
+            row[h]   = a.codes + r * blocks * kInt4BlockBytes;
+            scale[h] = {nullptr, (const uint16_t *) a.scale + r * groups, a.zero ? a.zero + r * groups : nullptr, 0, groups};
+        }
+    }
+};
 
-// One CTA: 16 weight rows against up to NT * 8 rows of x; its warps share the blocks of k and add up in shared memory in a fixed
-// order.  Inside a group the codes less their zero are integers, so the MMA's sums are those of x times integers; each group's sum
-// is scaled in 32 bits.
-template <typename T, int G, int NT>
-__global__ void __launch_bounds__(32 * kGemmWarps) int4_gemm_kernel(const Int4GemmArgs a) {
-    grid_dep_begin();
-    __shared__ float part[kGemmWarps][NT * 8][17];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (NT * 8);
-    const int blocks = (a.K + kKB - 1) / kKB, groups = (a.K + G - 1) / G;
-    const int ra = min(n0 + g, a.N - 1), rb = min(n0 + g + 8, a.N - 1);
-    const uint8_t *wa = a.codes + (int64_t) ra * blocks * kInt4BlockBytes, *wb = a.codes + (int64_t) rb * blocks * kInt4BlockBytes;
-    RowScale<kWInt4> sa{}, sb{};
-    sa.s4 = a.scale + (int64_t) ra * groups;
-    sb.s4 = a.scale + (int64_t) rb * groups;
-    sa.count = sb.count = groups;
-    if (a.zero != nullptr) {
-        sa.z4 = a.zero + (int64_t) ra * groups;
-        sb.z4 = a.zero + (int64_t) rb * groups;
+// Up to eight rows, as far as they fit into shared memory.
+template <int G> struct Int4TokenRows {
+    const Int4GemmArgs &a;
+    const uint8_t *row;
+    RowScale<kWInt4> scale[2];
+    __device__ __forceinline__ Int4TokenRows(const Int4GemmArgs &a) : a(a) {}
+    __device__ __forceinline__ void open(int tile, int) {
+        const int lane = threadIdx.x & 31, blocks = (a.K + kKB - 1) / kKB, groups = (a.K + G - 1) / G;
+        row = a.codes + (int64_t) min(tile * 16 + (lane & 15), a.N - 1) * blocks * kInt4BlockBytes;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t r = min(tile * 16 + (lane >> 2) + 8 * h, a.N - 1);
+            scale[h] = {nullptr, (const uint16_t *) a.scale + r * groups, a.zero ? a.zero + r * groups : nullptr, 0, groups};
+        }
     }
-    const T *x[NT];
-    bool live[NT];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        const int m = m0 + i * 8 + g;
-        live[i]     = m < a.M;
-        x[i]        = (const T *) a.x + (live[i] ? m : 0) * a.ldx + 8 * t;
-    }
-    float acc[NT][4];
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-    auto block = [&](int kb, const RowPiece<kWInt4> &pa, const RowPiece<kWInt4> &pb) {
-        few_rows_block<T, kWInt4, G, NT, 1>(acc, kb, pa, pb, sa, sb, [&](int i, int q, int) {
-            const int k = kb * kKB + 32 * q;
-            return live[i] && k + 8 * t < a.K ? *reinterpret_cast<const uint4 *>(x[i] + k) : make_uint4(0, 0, 0, 0);
-        });
-    };
-    constexpr int kAhead = 4; // blocks whose weights are in flight
-    for (int kb = warp; kb < blocks; kb += kGemmWarps * kAhead) {
-        RowPiece<kWInt4> pa[kAhead], pb[kAhead];
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-            if (kb + u * kGemmWarps < blocks) {
-                pa[u].load(wa, kb + u * kGemmWarps, t, a.K);
-                pb[u].load(wb, kb + u * kGemmWarps, t, a.K);
+};
+template <typename T, int G> __global__ void __launch_bounds__(32 * kTokenWarps, 1) int4_token_kernel(const __grid_constant__ Int4GemmArgs a, int shares) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int lane = threadIdx.x & 31, blocks = (a.K + kKB - 1) / kKB;
+    few_tokens_walk<T, kWInt4, G, 2, false, false, false>(
+        smem, a.M, (a.N + 15) / 16, shares, 1, a.K, Int4TokenRows<G>(a),
+        [&](uint8_t *x, uint8_t *runs) {
+            stage_blocks<T, T, kWInt4, G, 2>(x, runs, blocks, a.M, [&](int block, int col, int &left) {
+                left = a.K - block * kKB;
+                return (const T *) a.x + col * a.ldx + block * kKB;
+            });
+        },
+        [&](int tile, auto &&sum) {
+            for (int i = lane; i < a.M * 16; i += 32) {
+                const int m = i / 16, n = tile * 16 + i % 16;
+                if (n >= a.N) continue;
+                float v = sum(m, i % 16);
+                if (a.bias != nullptr) v += to_f32(((const T *) a.bias)[n]);
+                ((T *) a.out)[(int64_t) m * a.N + n] = from_f32<T>(v);
             }
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-            if (kb + u * kGemmWarps < blocks) block(kb + u * kGemmWarps, pa[u], pb[u]);
-    }
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        part[warp][i * 8 + 2 * t][g]         = acc[i][0];
-        part[warp][i * 8 + 2 * t + 1][g]     = acc[i][1];
-        part[warp][i * 8 + 2 * t][g + 8]     = acc[i][2];
-        part[warp][i * 8 + 2 * t + 1][g + 8] = acc[i][3];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < NT * 8 * 16; i += 32 * kGemmWarps) {
-        const int m = i / 16, n = i % 16;
-        if (m0 + m >= a.M || n0 + n >= a.N) continue;
-        float s = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kGemmWarps; ++w) s += part[w][m][n];
+        });
+}
+
+// More rows: a CTA has WR * 16 weight rows and up to NT * 8 rows of x; WK shares of k are added up in shared memory in a fixed order.
+template <int G> struct Int4BatchRows : Int4Rows<G> {
+    ScaledRows xs;
+    int row0;
+    __device__ __forceinline__ const uint8_t *x(int, int col) const { return xs.planes + (row0 + col) * xs.pitch; }
+    __device__ __forceinline__ const float *runs(int col) const { return xs.runs + (int64_t) (row0 + col) * xs.blocks; }
+};
+template <typename T, int G, int NT, int WR, int WK, int kStages>
+__global__ void __launch_bounds__(32 * WR * WK, 2) int4_gemm_kernel(const Int4GemmArgs a) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    using W = Walk<kWInt4, 128, WR, WK>;
+    const int n0 = blockIdx.x * W::kRows, m0 = blockIdx.y * (NT * 8), cols = min(NT * 8, a.M - m0);
+    Int4BatchRows<G> src;
+    src.aim(a, n0 + (threadIdx.x >> 5) % WR * 16);
+    src.xs   = a.xs;
+    src.row0 = m0;
+    float acc[NT][4] = {};
+    few_rows_walk<T, kWInt4, G, 128, NT, WR, WK, kStages, 1, false>(acc, smem, a.K, cols, (cols + 7) / 8, src);
+    const ShareSums<NT, WR, WK> sums(acc, smem);
+    for (int i = threadIdx.x; i < cols * W::kRows; i += W::kThreads) {
+        const int m = i / W::kRows, n = i % W::kRows;
+        if (n0 + n >= a.N) continue;
+        float s = sums.sum(m, n);
         if (a.bias != nullptr) s += to_f32(((const T *) a.bias)[n0 + n]);
         ((T *) a.out)[(int64_t) (m0 + m) * a.N + n0 + n] = from_f32<T>(s);
     }
 }
 
-template <typename T, int G> cudaError_t launch_gemm(const Int4GemmArgs &a, cudaStream_t st) {
-    const unsigned gx = (unsigned) cdiv(a.N, 16);
-    if (a.M <= 8) return launch_after(int4_gemm_kernel<T, G, 1>, dim3(gx, 1), 32 * kGemmWarps, 0, st, 1, a);
-    if (a.M <= 16) return launch_after(int4_gemm_kernel<T, G, 2>, dim3(gx, 1), 32 * kGemmWarps, 0, st, 1, a);
-    return launch_after(int4_gemm_kernel<T, G, 4>, dim3(gx, (unsigned) cdiv(a.M, 32)), 32 * kGemmWarps, 0, st, 1, a);
+template <typename T, int G, int NT, int WR, int WK, int kStages> cudaError_t launch_tile(const Int4GemmArgs &a, cudaStream_t st) {
+    using W = Walk<kWInt4, 128, WR, WK>;
+    const int smem = W::template smem<NT>(kStages, 1, (int) imin(a.M, NT * 8));
+    return launch_early(int4_gemm_kernel<T, G, NT, WR, WK, kStages>, dim3((unsigned) cdiv(a.N, W::kRows), (unsigned) cdiv(a.M, NT * 8)), W::kThreads,
+                        (size_t) smem, st, a);
+}
+
+constexpr int kMostSmem = 227 * 1024 - 1024; // of a CTA, less what is not dynamic
+
+template <typename T, int G> int launch_gemm(const Int4GemmArgs &a, cudaStream_t st) {
+    const int x_bytes = a.M <= kTokenCols && a.K <= 1 << 20 ? TokenX<kWInt4, G>::bytes(2, a.M, cdiv(a.K, kKB)) : kMostSmem;
+    if (token_smem(x_bytes, a.M) <= kMostSmem) {
+        int sms = 0;
+        if (int rc = sm_count(&sms)) return rc;
+        const int tiles = cdiv(a.N, 16), shares = token_shares(tiles, cdiv(a.K, kKB), sms);
+        PTB_CUDA(launch_early(int4_token_kernel<T, G>, dim3((unsigned) cdiv(tiles, kTokenWarps >> shares)), 32 * kTokenWarps, (size_t) token_smem(x_bytes, a.M), st, a, shares));
+        PTB_LAUNCH_CHECK("int4_token_kernel");
+        return 0;
+    }
+    const int64_t warps = a.M * cdiv<int64_t>(a.K, kKB);
+    PTB_CUDA(launch_early(scale_rows_kernel<T, kWInt4>, dim3((unsigned) cdiv<int64_t>(warps, 4)), 128, 0, st, (const T *) a.x, a.ldx, a.M, a.K, a.xs));
+    PTB_LAUNCH_CHECK("scale_rows_kernel");
+    if (a.M <= 8) PTB_CUDA((launch_tile<T, G, 1, 2, 4, 4>(a, st)));
+    else if (a.M <= 16) PTB_CUDA((launch_tile<T, G, 2, 4, 2, 4>(a, st)));
+    else PTB_CUDA((launch_tile<T, G, 4, 4, 2, 4>(a, st)));
+    PTB_LAUNCH_CHECK("int4_gemm_kernel");
+    return 0;
 }
 
 bool is_group(int64_t g) { return g == 32 || g == 64 || g == 128; }
@@ -224,6 +254,8 @@ bool is_group(int64_t g) { return g == 32 || g == 64 || g == 128; }
     }
 
 } // namespace
+
+int int4_status(int *status, int reset) { return few_status(status, reset); }
 } // namespace ptb
 
 using namespace ptb;
@@ -274,23 +306,26 @@ int ptb_dequant_int4(const void *codes, const void *scale, const void *zero, int
     return 0;
 }
 
+int64_t ptb_gemm_int4_workspace(int dtype, int64_t M, int64_t K, int64_t group) {
+    if (M < 0 || K < 1 || (dtype != PTB_BF16 && dtype != PTB_F16) || !is_group(group)) return -1;
+    return scaled_bytes(1, M, K, 128);
+}
+
 int ptb_gemm_int4(const void *x, int dtype, int64_t ldx, int64_t M, int64_t N, int64_t K, const void *codes, const void *scale, const void *zero,
-                  int64_t group, const void *bias, void *out, ptb_stream_t stream) {
+                  int64_t group, const void *bias, void *workspace, void *out, ptb_stream_t stream) {
     PTB_REQUIRE(M >= 0 && N >= 0 && K >= 1, PTB_ERR_ARG, "gemm_int4: bad shape");
     PTB_REQUIRE(dtype == PTB_BF16 || dtype == PTB_F16, PTB_ERR_ARG, "gemm_int4: x must be bf16 or fp16");
     PTB_REQUIRE(is_group(group), PTB_ERR_ARG, "gemm_int4: the group size must be 32, 64 or 128");
     PTB_REQUIRE(K % 8 == 0 && (M <= 1 || ldx % 8 == 0), PTB_ERR_ALIGN, "gemm_int4: the row length and pitch of x must be multiples of 8");
     PTB_REQUIRE(M <= 1 || ldx >= K, PTB_ERR_ARG, "gemm_int4: rows of x overlap");
-    PTB_REQUIRE(K <= 1 << 24 && N <= 1 << 30 && M <= 1 << 20, PTB_ERR_TOO_LARGE, "gemm_int4: matrix too large");
+    PTB_REQUIRE(K <= 1 << 24 && N <= 1 << 30 && M <= 1 << 20 && M * K <= 1ll << 34, PTB_ERR_TOO_LARGE, "gemm_int4: matrix too large");
     if (M == 0 || N == 0) return 0;
-    PTB_REQUIRE(x && codes && scale && out, PTB_ERR_ARG, "gemm_int4: null pointer");
-    PTB_REQUIRE(aligned16(x) && aligned16(codes), PTB_ERR_ALIGN, "gemm_int4: x and the codes must be 16-byte aligned");
-    const Int4GemmArgs a{x, ldx, (int) M, (int) N, (int) K, (const uint8_t *) codes, (const __nv_bfloat16 *) scale, (const uint8_t *) zero, bias, out};
-    PTB_SWITCH_INT4_GROUP(group, G, {
-        if (dtype == PTB_BF16) PTB_CUDA((launch_gemm<__nv_bfloat16, G>(a, (cudaStream_t) stream)));
-        else PTB_CUDA((launch_gemm<__half, G>(a, (cudaStream_t) stream)));
-    });
-    PTB_LAUNCH_CHECK("int4_gemm_kernel");
+    PTB_REQUIRE(x && codes && scale && workspace && out, PTB_ERR_ARG, "gemm_int4: null pointer");
+    PTB_REQUIRE(aligned16(x) && aligned16(codes) && aligned16(workspace), PTB_ERR_ALIGN, "gemm_int4: x, the codes and the workspace must be 16-byte aligned");
+    const Int4GemmArgs a{x, ldx, scaled_rows_at(workspace, 1, M, K), (int) M, (int) N, (int) K, (const uint8_t *) codes,
+                         (const __nv_bfloat16 *) scale, (const uint8_t *) zero, bias, out};
+    cudaStream_t st = (cudaStream_t) stream;
+    PTB_SWITCH_INT4_GROUP(group, G, return dtype == PTB_BF16 ? launch_gemm<__nv_bfloat16, G>(a, st) : launch_gemm<__half, G>(a, st));
     return 0;
 }
 

@@ -2,18 +2,21 @@
 //   y[t] = sum_j p[t, j] * W2[e] (silu(W1[e] x_t, first half) * (W1[e] x_t, second half)),  e = ids[t, j]
 // from weights as they are kept: 16-bit, FP8 with inverse scales, or 4-bit groups.
 //
-// Three kernels: a list of the experts that are hit and their tokens, gate + up projection with the activation, down projection
-// with the weighted sum over a token's experts.  What bounds them is reading the weights of the experts that are hit, once.
+// What bounds it is reading the weights of the experts that are hit, once.  For a token or a few (at most 8 tokens and 32 (token,
+// expert) pairs, as far as x and h fit into shared memory) two kernels, whose CTAs find the pairs of the experts themselves:
 //
-//  * moe_gate_up_kernel: one CTA per eight channels of one hit expert: the 16 rows of its MMAs are eight gate rows and the eight up
-//    rows that go with them, so both halves of a channel meet in one lane and the activation needs no exchange.  Its warps share k.
-//  * moe_down_kernel: one CTA per 16 output columns, over all experts that are hit: its warps share the list of (expert, block of k)
-//    and keep one 32-bit sum per token and column each, added up in a fixed order at the end.  Nothing is added in memory, so no
-//    atomics, no second pass, and the same result every time.
+//  * moe_gate_up_token_kernel: the 16 rows of a tile are eight gate rows and the eight up rows that go with them, so both halves of a
+//    channel are put together at the end of a tile.  The activation h is weighted with p there.
+//  * moe_down_token_kernel: a tile is 16 output columns of all experts, whose blocks of k are one long k; the eight columns of the
+//    MMA are the tokens.  Nothing is added in memory: no atomics, no second pass, and the same bits every time.
 //
-// The activation h between the two is kept as a sum of two bf16 (16 bits of mantissa): its rounding is not felt in the result, and
-// the second MMA costs nothing next to the weights.
-#include "ptb_few_rows.cuh"
+// For more tokens four: moe_list_kernel sorts the pairs by expert, beside the scaling of x; moe_gate_up_kernel on an expert's own tokens;
+// moe_down_kernel writes a 32-bit row per pair and moe_merge_kernel adds up a token's rows in the router's order.
+//
+// The activation h between the two products is kept in 32 bits and then scaled like x, or scaled at once, per 64 channels: to fp16
+// (2^-12 of each value; with fp16 results what that leaves is a second term), for 4-bit weights and few tokens to 16-bit integers.  With
+// 16-bit weights it is two bf16 (2^-17).  Its rounding is not felt in the result.
+#include "ptb_few_tokens.cuh"
 
 namespace ptb {
 namespace {
@@ -37,7 +40,7 @@ template <int FMT> __device__ __forceinline__ RowScale<FMT> row_scale(const Expe
     RowScale<FMT> r{};
     if constexpr (FMT == kWInt4) {
         const int64_t at = (e * rows + row) * w.groups;
-        r.s4    = (const __nv_bfloat16 *) w.scale + at;
+        r.s4    = (const uint16_t *) w.scale + at;
         r.z4    = w.zero != nullptr ? w.zero + at : nullptr;
         r.count = w.groups;
     } else if constexpr (FMT != kW16) {
@@ -53,16 +56,28 @@ struct Lists {
     int *first;      // [a]: its first slot; [number hit]: slots in all
     int *token;      // of a slot
     float *prob;     // of a slot
+    int *slot;       // of a pair; -1 where it has none
 };
-__host__ __device__ inline int64_t list_words(int64_t pairs) { return 1 + pairs + (pairs + 1) + pairs + pairs; }
+__host__ __device__ inline int64_t list_words(int64_t pairs) { return 1 + pairs + (pairs + 1) + pairs + pairs + pairs; }
 __host__ __device__ inline Lists lists_at(void *ws, int64_t pairs) {
     int *p = (int *) ws;
-    return {p, p + 1 + pairs, p + 2 + 2 * pairs, (float *) (p + 2 + 3 * pairs)};
+    return {p, p + 1 + pairs, p + 2 + 2 * pairs, (float *) (p + 2 + 3 * pairs), p + 2 + 4 * pairs};
 }
 
 // A token that names an expert twice has one slot with the sum of the two probabilities.  Ids outside [0, E) have none.
-__global__ void __launch_bounds__(1024) moe_list_kernel(const int64_t *ids, const float *probs, int T, int k, int E, Lists out) {
-    grid_dep_begin();
+// CTAs from 1 on split x, if there are any.
+template <typename X, int FMT>
+__global__ void __launch_bounds__(1024) moe_list_kernel(const int64_t *ids, const float *probs, int T, int k, int E, Lists out, const X *x, int64_t ldx, int H,
+                                                        const ScaledRows terms) {
+    grid_dep_wait();
+    grid_dep_open();
+    if (blockIdx.x > 0) {
+        if constexpr (kScaledX<FMT>) {
+            const int blocks = (H + kKB - 1) / kKB, i = (blockIdx.x - 1) * 32 + (threadIdx.x >> 5);
+            if (i < T * blocks) scale_block<X, FMT>(x + i / blocks * ldx, H, i % blocks, i / blocks, terms);
+        }
+        return;
+    }
     __shared__ int count[kMaxExperts];
     __shared__ short id[kMaxPairs];
     __shared__ int warp_hit[32], warp_slots[32];
@@ -123,6 +138,9 @@ __global__ void __launch_bounds__(1024) moe_list_kernel(const int64_t *ids, cons
             const int slot  = count[e] + __popc(same & ((1u << lane) - 1));
             out.token[slot] = i / k;
             out.prob[slot]  = prob[i];
+            out.slot[i]     = slot;
+        } else if (i < n) {
+            out.slot[i] = -1;
         }
         __syncwarp();
         if (e >= 0 && (same >> lane) == 1u) count[e] += __popc(same); // the last lane of each expert
@@ -130,235 +148,393 @@ __global__ void __launch_bounds__(1024) moe_list_kernel(const int64_t *ids, cons
     }
 }
 
-struct GateUpArgs {
+struct LayerArgs {
     const void *x;
     int64_t ldx;
-    int H, I;
-    ExpertWeight w;
-    Lists lists;
-    __nv_bfloat16 *h_hi, *h_lo; // [slots, I]
+    int T, k, E, H, I;
+    const int64_t *ids;
+    const float *probs;
+    ExpertWeight w1, w2;
+    float *h32;                 // two kernels: [pairs, I], at the first pair with this token and expert
+    Lists lists;                // four kernels:
+    ScaledRows xs, hs;          // x [T, H] and h [slots, I], or with 16-bit weights
+    __nv_bfloat16 *h_hi, *h_lo; // h in two parts
+    float *rows;                // [slots, H]
+    void *out;
 };
 
-constexpr int kGateUpWarps = 8;
+// ---- a token or a few -----------------------------------------------------------------------------------------------------------
+constexpr int kTokenPairs = 32;
 
-template <typename T, int FMT, int G, int NT>
-__global__ void __launch_bounds__(32 * kGateUpWarps) moe_gate_up_kernel(const GateUpArgs a) {
-    grid_dep_begin();
+// Which experts are hit, and at which pair each has its h for each token (-1: none), with what weight.
+struct Pairs {
+    int hits;
+    int expert[kTokenPairs];
+    signed char slot[kTokenPairs * kTokenCols];
+    float weight[kTokenPairs * kTokenCols];
+};
+// Called by one warp; lane i has pair i.
+__device__ __forceinline__ void find_pairs(const LayerArgs &a, Pairs &out) {
+    const int lane = threadIdx.x & 31, n = a.T * a.k;
+    int e = -1;
+    float p = 0.0f;
+    if (lane < n) {
+        const int64_t id = a.ids[lane];
+        if (id >= 0 && id < a.E) {
+            e = (int) id;
+            p = a.probs[lane];
+        }
+    }
+    const unsigned same = __match_any_sync(0xffffffffu, e);
+    const bool first = e >= 0 && __ffs((int) same) - 1 == lane;
+    const unsigned firsts = __ballot_sync(0xffffffffu, first);
+    const int hit = __popc(firsts & ((1u << (__ffs((int) same) - 1)) - 1)); // of the expert of this lane's pair
+    if (first) out.expert[hit] = e;
+    if (lane == 0) out.hits = __popc(firsts);
+    // a token that names an expert twice has it once, with the sum of the two weights
+    const unsigned own = (unsigned) ((1ull << a.k) - 1);
+#pragma unroll 1
+    for (int c = 0; c < a.T; ++c) {
+        const unsigned mine = same >> (c * a.k) & own;
+        float sum = 0.0f;
+#pragma unroll 1
+        for (unsigned left = __reduce_or_sync(0xffffffffu, first ? mine : 0u); left != 0; left &= left - 1) {
+            const int j   = __ffs((int) left) - 1;
+            const float v = __shfl_sync(0xffffffffu, p, c * a.k + j);
+            if (mine >> j & 1) sum += v;
+        }
+        if (first) {
+            out.slot[hit * kTokenCols + c]   = (signed char) (mine == 0 ? -1 : c * a.k + __ffs((int) mine) - 1);
+            out.weight[hit * kTokenCols + c] = sum;
+        }
+    }
+}
+
+template <int FMT> struct ExpertRows { // a lane's two rows of an expert's weight
+    const uint8_t *row[2];
+    RowScale<FMT> scale[2];
+    __device__ __forceinline__ void aim(const ExpertWeight &w, int64_t e, int r0, int r1, int rows) {
+        row[0]   = w.data + e * w.expert_bytes + r0 * w.row_bytes;
+        row[1]   = w.data + e * w.expert_bytes + r1 * w.row_bytes;
+        scale[0] = row_scale<FMT>(w, e, r0, rows);
+        scale[1] = row_scale<FMT>(w, e, r1, rows);
+    }
+};
+
+template <int FMT> struct TokenRows { // row lane % 16 of a tile, and the scales of rows lane / 4 and lane / 4 + 8
+    const uint8_t *row;
+    RowScale<FMT> scale[2];
+};
+template <int FMT> struct GateUpTokenRows : TokenRows<FMT> {
+    const LayerArgs &a;
+    const Pairs &pairs;
+    int tiles; // of an expert
+    __device__ __forceinline__ GateUpTokenRows(const LayerArgs &a, const Pairs &pairs, int tiles) : a(a), pairs(pairs), tiles(tiles) {}
+    __device__ __forceinline__ void open(int tile, int) {
+        const int hit = tile / tiles, r0 = (tile - hit * tiles) * 8, lane = threadIdx.x & 31, r = min(r0 + (lane >> 2), a.I - 1);
+        const int64_t e = pairs.expert[hit];
+        this->row = a.w1.data + e * a.w1.expert_bytes + (min(r0 + (lane & 7), a.I - 1) + (lane & 8 ? a.I : 0)) * a.w1.row_bytes;
+        this->scale[0] = row_scale<FMT>(a.w1, e, r, 2 * a.I);
+        this->scale[1] = row_scale<FMT>(a.w1, e, a.I + r, 2 * a.I);
+    }
+};
+
+template <typename T, int FMT, int G>
+__global__ void __launch_bounds__(32 * kTokenWarps, 1) moe_gate_up_token_kernel(const __grid_constant__ LayerArgs a, int shares) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ Pairs pairs;
+    grid_dep_wait(); // the kernel before this one is somebody else's
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tiles = (a.I + 7) / 8, blocks = (a.H + kKB - 1) / kKB;
+    constexpr int kTerms = FMT == kWInt4 ? 2 : 1;
+    if (warp == 0) find_pairs(a, pairs);
+    __syncthreads();
+    few_tokens_walk<T, FMT, G, kTerms, false, false, false>(
+        smem, a.T, pairs.hits * tiles, shares, 1, a.H, GateUpTokenRows<FMT>(a, pairs, tiles),
+        [&](uint8_t *x, uint8_t *runs) {
+            stage_blocks<T, T, FMT, G, kTerms>(x, runs, blocks, a.T, [&](int block, int col, int &left) {
+                left = a.H - block * kKB;
+                return (const T *) a.x + col * a.ldx + block * kKB;
+            });
+        },
+        [&](int tile, auto &&sum) {
+            const int hit = tile / tiles, r0 = (tile - hit * tiles) * 8;
+            for (int i = lane; i < a.T * 8; i += 32) {
+                const int c = i / 8, r = i % 8, slot = pairs.slot[hit * kTokenCols + c];
+                if (slot >= 0 && r0 + r < a.I) a.h32[(int64_t) slot * a.I + r0 + r] = swiglu_prob(sum(c, r), sum(c, r + 8), pairs.weight[hit * kTokenCols + c]);
+            }
+        });
+}
+
+template <int FMT> struct DownTokenRows : TokenRows<FMT> {
+    const LayerArgs &a;
+    const Pairs &pairs;
+    __device__ __forceinline__ DownTokenRows(const LayerArgs &a, const Pairs &pairs) : a(a), pairs(pairs) {}
+    __device__ __forceinline__ void open(int tile, int segment) {
+        const int lane = threadIdx.x & 31, r = tile * 16 + (lane >> 2);
+        const int64_t e = pairs.expert[segment];
+        this->row = a.w2.data + e * a.w2.expert_bytes + min(tile * 16 + (lane & 15), a.H - 1) * a.w2.row_bytes;
+        this->scale[0] = row_scale<FMT>(a.w2, e, min(r, a.H - 1), a.H);
+        this->scale[1] = row_scale<FMT>(a.w2, e, min(r + 8, a.H - 1), a.H);
+    }
+    __device__ __forceinline__ bool mask(int segment, int column) const { return pairs.slot[segment * kTokenCols + column] >= 0; }
+};
+
+template <typename T> constexpr int kHScaled = std::is_same<T, __half>::value ? 2 : 1; // terms of scaled h
+template <typename T, int FMT> constexpr int kHTerms = FMT == kW16 || FMT == kWInt4 || std::is_same<T, __half>::value ? 2 : 1;
+
+template <typename T, int FMT, int G>
+__global__ void __launch_bounds__(32 * kTokenWarps, 1) moe_down_token_kernel(const __grid_constant__ LayerArgs a, int shares) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ Pairs pairs;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, blocks = (a.I + kKB - 1) / kKB;
+    // 16-bit weights: the MMA's type is that of h, bf16, whatever x is
+    using M = __nv_bfloat16;
+    constexpr int kTerms = kHTerms<T, FMT>;
+    if (warp == 0) find_pairs(a, pairs);
+    __syncthreads();
+    few_tokens_walk<M, FMT, G, kTerms, FMT == kW16 && std::is_same<T, __half>::value, true, true>(
+        smem, a.T, (a.H + 15) / 16, shares, pairs.hits, a.I, DownTokenRows<FMT>(a, pairs),
+        [&](uint8_t *x, uint8_t *runs) {
+            stage_blocks<M, float, FMT, G, kTerms>(x, runs, pairs.hits * blocks, a.T, [&](int block, int col, int &left) {
+                const int hit = block / blocks, kb = block - hit * blocks, slot = pairs.slot[hit * kTokenCols + col];
+                left = slot < 0 ? 0 : a.I - kb * kKB; // zeros for a token that does not go there
+                return a.h32 + (int64_t) max(slot, 0) * a.I + kb * kKB;
+            });
+        },
+        [&](int tile, auto &&sum) {
+            for (int i = lane; i < a.T * 16; i += 32) {
+                const int m = i / 16, n = tile * 16 + i % 16;
+                if (n < a.H) ((T *) a.out)[(int64_t) m * a.H + n] = from_f32<T>(sum(m, i % 16));
+            }
+        });
+}
+
+// ---- more tokens: gate and up projection -----------------------------------------------------------------------------------------
+constexpr int kChannels = 64; // of a CTA: eight warps of eight
+
+template <int FMT> struct GateUpRows : ExpertRows<FMT> {
+    const uint8_t *x0;
+    int64_t pitch;
+    const float *runs0;
+    int blocks;
+    const int *token; // row of x of a column
+    __device__ __forceinline__ const uint8_t *x(int, int col) const { return x0 + token[col] * pitch; }
+    __device__ __forceinline__ const float *runs(int col) const { return runs0 + (int64_t) token[col] * blocks; }
+};
+
+// blockIdx.y counts the experts that are hit.
+template <typename T, int FMT, int G, int NT, int kStages>
+__global__ void __launch_bounds__(256, 2) moe_gate_up_kernel(const LayerArgs a) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    using W = Walk<FMT, 128, 8, 1>;
+    constexpr int kPitch = kChannels + 1;
+    __shared__ int token[NT * 8];
+    __shared__ float h_of[kScaledX<FMT> ? NT * 8 * kPitch : 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
+    grid_dep_wait();
     const int hit = blockIdx.y;
     if (hit >= a.lists.active[0]) return;
-    __shared__ float part[kGateUpWarps][NT * 8][17];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int r0 = blockIdx.x * 8, row = min(r0 + g, a.I - 1);
     const int64_t e = a.lists.active[1 + hit];
     const int begin = a.lists.first[hit], end = a.lists.first[hit + 1];
-    const uint8_t *wa = a.w.data + e * a.w.expert_bytes + row * a.w.row_bytes, *wb = wa + (int64_t) a.I * a.w.row_bytes;
-    const RowScale<FMT> sa = row_scale<FMT>(a.w, e, row, 2 * a.I), sb = row_scale<FMT>(a.w, e, a.I + row, 2 * a.I);
-    const int blocks = (a.H + kKB - 1) / kKB;
-    constexpr int kAhead = FMT == kWInt4 ? 4 : FMT == kW16 ? 1 : 2;
+    const int r0 = blockIdx.x * kChannels, row = min(r0 + warp * 8 + g, a.I - 1);
+    GateUpRows<FMT> src;
+    src.aim(a.w1, e, row, a.I + row, 2 * a.I);
+    src.x0     = kScaledX<FMT> ? a.xs.planes : (const uint8_t *) a.x;
+    src.pitch  = kScaledX<FMT> ? a.xs.pitch : a.ldx * 2;
+    src.runs0  = a.xs.runs;
+    src.blocks = a.xs.blocks;
+    src.token  = token;
     for (int s0 = begin; s0 < end; s0 += NT * 8) {
-        const T *x[NT];
-        bool live[NT];
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            const int s = s0 + i * 8 + g;
-            live[i]     = s < end;
-            x[i]        = (const T *) a.x + (live[i] ? a.lists.token[s] : 0) * a.ldx;
+        const int cols = min(NT * 8, end - s0);
+        if (threadIdx.x < cols) token[threadIdx.x] = a.lists.token[s0 + threadIdx.x];
+        __syncthreads();
+        float acc[NT][4] = {};
+        if (r0 < a.I) few_rows_walk<T, FMT, G, 128, NT, 8, 1, kStages, 1, false>(acc, smem, a.H, cols, (cols + 7) / 8, src);
+        else grid_dep_open(); // (past the last channel there is only h's padding to write)
+        const ShareSums<NT, 8, 1> sums(acc, smem);
+        for (int i = threadIdx.x; i < cols * kChannels; i += W::kThreads) {
+            const int c = i / kChannels, r = i % kChannels, at = r / 8 * 16 + r % 8, slot = s0 + c;
+            const float h = r0 + r < a.I ? swiglu_prob(sums.sum(c, at), sums.sum(c, at + 8), a.lists.prob[slot]) : 0.0f;
+            if constexpr (kScaledX<FMT>) {
+                h_of[c * kPitch + r] = h;
+            } else if (r0 + r < a.I) {
+                const __nv_bfloat16 hi = __float2bfloat16_rn(h);
+                a.h_hi[(int64_t) slot * a.I + r0 + r] = hi;
+                a.h_lo[(int64_t) slot * a.I + r0 + r] = __float2bfloat16_rn(fabsf(h) < INFINITY ? h - __bfloat162float(hi) : 0.0f);
+            }
         }
-        float acc[NT][4];
+        if constexpr (kScaledX<FMT>) { // a half-warp scales a token's 64 channels, four a lane
+            __syncthreads();
+            for (int c2 = warp; 2 * c2 < cols; c2 += 8) {
+                const int c = min(2 * c2 + (lane >> 4), cols - 1), in = (lane & 15) * 4;
+                const int64_t slot = s0 + c;
+                float v[4], largest = 0.0f, scale, inv;
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-        for (int kb = warp; kb < blocks; kb += kGateUpWarps * kAhead) {
-            RowPiece<FMT> pa[kAhead], pb[kAhead];
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u)
-                if (kb + u * kGateUpWarps < blocks) {
-                    pa[u].load(wa, kb + u * kGateUpWarps, t, a.H);
-                    pb[u].load(wb, kb + u * kGateUpWarps, t, a.H);
+                for (int j = 0; j < 4; ++j) {
+                    v[j] = h_of[c * kPitch + in + j];
+                    if (fabsf(v[j]) < INFINITY) largest = fmaxf(largest, fabsf(v[j]));
                 }
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int b = kb + u * kGateUpWarps;
-                if (b < blocks)
-                    few_rows_block<T, FMT, G, NT, 1>(acc, b, pa[u], pb[u], sa, sb, [&](int i, int q, int) {
-                        const int k = b * kKB + octet_k<FMT>(q, t);
-                        return live[i] && k < a.H ? *reinterpret_cast<const uint4 *>(x[i] + k) : make_uint4(0, 0, 0, 0);
-                    });
+                for (int o = 8; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+                block_scale(largest, kTopHalf, scale, inv);
+                uint8_t *to = a.hs.planes + slot * a.hs.pitch + (r0 + in) * 2;
+#pragma unroll
+                for (int term = 0; term < kHScaled<T>; ++term) {
+                    __half h[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float s = v[j] * inv;
+                        h[half_place<FMT>(j)] = term == 0 ? __float2half_rn(s) : __float2half_rn(fabsf(s) < INFINITY ? s - __half2float(__float2half_rn(s)) : 0.0f);
+                    }
+                    uint2 u;
+                    memcpy(&u, h, 8);
+                    *reinterpret_cast<uint2 *>(to + term * a.hs.plane) = u;
+                }
+                if ((lane & 15) == 0) a.hs.runs[slot * a.hs.blocks * 2 + r0 / 64] = scale;
             }
         }
-        __syncthreads(); // the sums of the eights before are read
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            part[warp][i * 8 + 2 * t][g]         = acc[i][0];
-            part[warp][i * 8 + 2 * t + 1][g]     = acc[i][1];
-            part[warp][i * 8 + 2 * t][g + 8]     = acc[i][2];
-            part[warp][i * 8 + 2 * t + 1][g + 8] = acc[i][3];
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < NT * 64; i += 32 * kGateUpWarps) {
-            const int m = i / 8, r = i % 8;
-            if (s0 + m >= end || r0 + r >= a.I) continue;
-            float gate = 0.0f, up = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kGateUpWarps; ++w) {
-                gate += part[w][m][r];
-                up += part[w][m][r + 8];
-            }
-            const float h = swiglu_prob(gate, up, 1.0f);
-            const __nv_bfloat16 hi = __float2bfloat16_rn(h);
-            const float rest = h - __bfloat162float(hi);
-            const int64_t at = (int64_t) (s0 + m) * a.I + r0 + r;
-            a.h_hi[at] = hi;
-            a.h_lo[at] = __float2bfloat16_rn(fabsf(h) < INFINITY ? rest : 0.0f);
-        }
+        if (s0 + NT * 8 < end) __syncthreads(); // all of this is read before it is written again
     }
 }
 
-struct DownArgs {
-    int T, H, I;
-    ExpertWeight w;
-    Lists lists;
-    const __nv_bfloat16 *h_hi, *h_lo;
-    void *out; // [T, H]
+// ---- more tokens: down projection, a row per pair --------------------------------------------------------------------------------
+template <int FMT> struct DownRows : ExpertRows<FMT> {
+    const uint8_t *x0;
+    int64_t plane, pitch;
+    const float *runs0;
+    int blocks;
+    __device__ __forceinline__ const uint8_t *x(int term, int col) const { return x0 + term * plane + col * pitch; }
+    __device__ __forceinline__ const float *runs(int col) const { return runs0 + (int64_t) col * blocks * 2; }
 };
 
-constexpr int kDownWarps = 16;
-
-template <typename T, int FMT, int G, int NT>
-__global__ void __launch_bounds__(32 * kDownWarps) moe_down_kernel(const DownArgs a) {
-    grid_dep_begin();
-    extern __shared__ float sums[]; // [warp][token][17]
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int n0 = blockIdx.x * 16, ra = min(n0 + g, a.H - 1), rb = min(n0 + g + 8, a.H - 1);
-    float *mine = sums + (int64_t) warp * a.T * 17;
-    for (int i = lane; i < a.T * 17; i += 32) mine[i] = 0.0f;
-    __syncwarp();
-    const int hits = a.lists.active[0], blocks = (a.I + kKB - 1) / kKB, total = hits * blocks;
-    const int last = (int) ((int64_t) (warp + 1) * total / kDownWarps);
-    using M = __nv_bfloat16; // the MMA's type: h is bf16 here whatever x is
-    // fp16 weights become the sum of two bf16, exactly
-    constexpr bool kSplit = FMT == kW16 && std::is_same<T, __half>::value;
-    for (int item = (int) ((int64_t) warp * total / kDownWarps); item < last;) {
-        const int hit = item / blocks, from = item - hit * blocks, to = min(blocks, from + last - item);
-        item += to - from;
-        const int64_t e = a.lists.active[1 + hit];
-        const int begin = a.lists.first[hit], end = a.lists.first[hit + 1];
-        const uint8_t *wa = a.w.data + e * a.w.expert_bytes + ra * a.w.row_bytes, *wb = a.w.data + e * a.w.expert_bytes + rb * a.w.row_bytes;
-        const RowScale<FMT> sa = row_scale<FMT>(a.w, e, ra, a.H), sb = row_scale<FMT>(a.w, e, rb, a.H);
-        constexpr int kAhead = FMT == kWInt4 ? 4 : FMT == kW16 ? 1 : 2;
-        for (int s0 = begin; s0 < end; s0 += NT * 8) {
-            int64_t row[NT];
-            bool live[NT];
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                const int s = s0 + i * 8 + g;
-                live[i]     = s < end;
-                row[i]      = (int64_t) (live[i] ? s : begin) * a.I;
-            }
-            float acc[NT][4];
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-            for (int kb = from; kb < to; kb += kAhead) {
-                RowPiece<FMT> pa[kAhead], pb[kAhead];
-#pragma unroll
-                for (int u = 0; u < kAhead; ++u)
-                    if (kb + u < to) {
-                        pa[u].load(wa, kb + u, t, a.I);
-                        pb[u].load(wb, kb + u, t, a.I);
-                    }
-#pragma unroll
-                for (int u = 0; u < kAhead; ++u) {
-                    const int b = kb + u;
-                    if (b >= to) break;
-                    auto x = [&](int i, int q, int term) {
-                        const int k = b * kKB + octet_k<FMT>(q, t);
-                        const __nv_bfloat16 *h = (term == 0 ? a.h_hi : a.h_lo) + row[i] + k;
-                        return live[i] && k < a.I ? *reinterpret_cast<const uint4 *>(h) : make_uint4(0, 0, 0, 0);
-                    };
-                    if constexpr (!kSplit) {
-                        few_rows_block<M, FMT, G, NT, 2>(acc, b, pa[u], pb[u], sa, sb, x);
-                    } else {
-                        RowPiece<FMT> ha, hb, la, lb;
-                        auto split = [](const RowPiece<FMT> &p, RowPiece<FMT> &hi, RowPiece<FMT> &lo) {
-#pragma unroll
-                            for (int v = 0; v < RowPiece<FMT>::kVecs; ++v) {
-                                const __half2 *f = reinterpret_cast<const __half2 *>(&p.v[v]);
-                                __nv_bfloat162 h2[4], l2[4];
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    const float2 w = __half22float2(f[j]);
-                                    h2[j] = __float22bfloat162_rn(w);
-                                    const float2 r = __bfloat1622float2(h2[j]);
-                                    l2[j] = __float22bfloat162_rn(make_float2(fabsf(w.x) < INFINITY ? w.x - r.x : 0.0f, fabsf(w.y) < INFINITY ? w.y - r.y : 0.0f));
-                                }
-                                memcpy(&hi.v[v], h2, 16);
-                                memcpy(&lo.v[v], l2, 16);
-                            }
-                        };
-                        split(pa[u], ha, la);
-                        split(pb[u], hb, lb);
-                        few_rows_block<M, FMT, G, NT, 2>(acc, b, ha, hb, sa, sb, x);
-                        few_rows_block<M, FMT, G, NT, 1>(acc, b, la, lb, sa, sb, x);
-                    }
-                }
-            }
-            // a slot's token and probability; a token has one slot an expert, so no two lanes add to one place
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int s = s0 + i * 8 + 2 * t + c;
-                    if (s < end) {
-                        float *to_add = mine + a.lists.token[s] * 17;
-                        const float p = a.lists.prob[s];
-                        to_add[g] += p * acc[i][c];
-                        to_add[g + 8] += p * acc[i][2 + c];
-                    }
-                }
-            __syncwarp();
-        }
+template <typename T, int FMT, int G, int NT, int kStages>
+__global__ void __launch_bounds__(256, 2) moe_down_kernel(const LayerArgs a) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    using W = Walk<FMT, 64, 8, 1>;
+    const int hit = blockIdx.y; // the lists are from two kernels before
+    if (hit >= a.lists.active[0]) {
+        grid_dep_wait();
+        return;
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < a.T * 16; i += 32 * kDownWarps) {
-        const int m = i / 16, n = i % 16;
-        if (n0 + n >= a.H) continue;
-        float s = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kDownWarps; ++w) s += sums[((int64_t) w * a.T + m) * 17 + n];
-        ((T *) a.out)[(int64_t) m * a.H + n0 + n] = from_f32<T>(s);
+    const int warp = threadIdx.x >> 5, g = (threadIdx.x & 31) >> 2;
+    const int64_t e = a.lists.active[1 + hit];
+    const int begin = a.lists.first[hit], end = a.lists.first[hit + 1];
+    const int n0 = blockIdx.x * W::kRows, row = n0 + warp * 16 + g;
+    DownRows<FMT> src;
+    src.aim(a.w2, e, min(row, a.H - 1), min(row + 8, a.H - 1), a.H);
+    src.plane  = kScaledX<FMT> ? a.hs.plane : (int64_t) ((const uint8_t *) a.h_lo - (const uint8_t *) a.h_hi);
+    src.pitch  = kScaledX<FMT> ? a.hs.pitch : (int64_t) a.I * 2;
+    src.blocks = a.hs.blocks;
+    for (int s0 = begin; s0 < end; s0 += NT * 8) {
+        const int cols = min(NT * 8, end - s0);
+        src.x0    = (kScaledX<FMT> ? a.hs.planes : (const uint8_t *) a.h_hi) + s0 * src.pitch;
+        src.runs0 = a.hs.runs + (int64_t) s0 * src.blocks * 2;
+        float acc[NT][4] = {};
+        few_rows_walk<__nv_bfloat16, FMT, G, 64, NT, 8, 1, kStages, kScaledX<FMT> ? kHScaled<T> : 2, FMT == kW16 && std::is_same<T, __half>::value>(
+            acc, smem, a.I, cols, (cols + 7) / 8, src);
+        const ShareSums<NT, 8, 1> sums(acc, smem);
+        for (int i = threadIdx.x; i < cols * W::kRows; i += W::kThreads) {
+            const int c = i / W::kRows, n = i % W::kRows;
+            if (n0 + n < a.H) a.rows[(int64_t) (s0 + c) * a.H + n0 + n] = sums.sum(c, n);
+        }
+        if (s0 + NT * 8 < end) __syncthreads();
     }
 }
 
-template <typename T, int FMT, int G, int NT>
-int launch_layer(const GateUpArgs &u, const DownArgs &d, int max_hits, cudaStream_t st) {
-    PTB_CUDA(launch_after(moe_gate_up_kernel<T, FMT, G, NT>, dim3((unsigned) cdiv(u.I, 8), (unsigned) max_hits), 32 * kGateUpWarps, 0, st, 1, u));
-    PTB_LAUNCH_CHECK("moe_gate_up_kernel");
-    const size_t smem = sizeof(float) * kDownWarps * d.T * 17;
-    auto down = moe_down_kernel<T, FMT, G, NT>;
-    if (smem > 48 * 1024) PTB_CUDA(cudaFuncSetAttribute(down, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
-    PTB_CUDA(launch_after(down, dim3((unsigned) cdiv(d.H, 16)), 32 * kDownWarps, smem, st, 1, d));
-    PTB_LAUNCH_CHECK("moe_down_kernel");
+// out[t] = the sum of token t's rows; one thread per eight columns
+template <typename T> __global__ void __launch_bounds__(128) moe_merge_kernel(const LayerArgs a) {
+    grid_dep_wait();
+    grid_dep_open();
+    const int n = (blockIdx.x * 128 + threadIdx.x) * 8, token = blockIdx.y;
+    if (n >= a.H) return;
+    float s[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] = 0.0f;
+    for (int j = 0; j < a.k; ++j) {
+        const int slot = a.lists.slot[token * a.k + j];
+        if (slot < 0) continue;
+        const float4 *r = reinterpret_cast<const float4 *>(a.rows + (int64_t) slot * a.H + n);
+        const float4 u = r[0], v = r[1];
+        s[0] += u.x; s[1] += u.y; s[2] += u.z; s[3] += u.w;
+        s[4] += v.x; s[5] += v.y; s[6] += v.z; s[7] += v.w;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ((T *) a.out)[(int64_t) token * a.H + n + j] = from_f32<T>(s[j]);
+}
+
+#define PTB_EARLY(name, kernel, ...)                         do {                                                         PTB_CUDA(launch_early(kernel, __VA_ARGS__));             PTB_LAUNCH_CHECK(name);                              } while (0)
+
+constexpr int kMostSmem = 227 * 1024 - 4096; // of a CTA, less what is not dynamic
+
+// Whether the two-kernel form has room for x and for h, and the shared memory of its kernels.
+template <typename T, int FMT, int G> bool fits_token(const LayerArgs &a, int &up, int &down) {
+    if (a.T > kTokenCols || a.T * a.k > kTokenPairs || a.H > 1 << 17 || a.I > 1 << 15) return false;
+    up   = token_smem(TokenX<FMT, G>::bytes(FMT == kWInt4 ? 2 : 1, a.T, cdiv(a.H, kKB)), a.T);
+    down = token_smem(TokenX<FMT, G>::bytes(kHTerms<T, FMT>, a.T, (int) imin(a.E, a.T * a.k) * cdiv(a.I, kKB)), a.T);
+    return up <= kMostSmem && down <= kMostSmem;
+}
+
+template <typename T, int FMT, int G> int launch_token(const LayerArgs &a, int up, int down, cudaStream_t st) {
+    int sms = 0;
+    if (int rc = sm_count(&sms)) return rc;
+    const int hits = (int) imin(a.E, a.T * a.k), up_tiles = hits * cdiv(a.I, 8), down_tiles = cdiv(a.H, 16);
+    const int up_shares = token_shares(up_tiles, cdiv(a.H, kKB), sms), down_shares = token_shares(down_tiles, hits * cdiv(a.I, kKB), sms);
+    const dim3 g1((unsigned) cdiv(up_tiles, kTokenWarps >> up_shares)), g2((unsigned) cdiv(down_tiles, kTokenWarps >> down_shares));
+    PTB_CUDA(launch_early(moe_gate_up_token_kernel<T, FMT, G>, g1, 32 * kTokenWarps, (size_t) up, st, a, up_shares));
+    PTB_LAUNCH_CHECK("moe_gate_up_token_kernel");
+    PTB_CUDA(launch_early(moe_down_token_kernel<T, FMT, G>, g2, 32 * kTokenWarps, (size_t) down, st, a, down_shares));
+    PTB_LAUNCH_CHECK("moe_down_token_kernel");
     return 0;
 }
 
-template <typename T, int FMT, int G> int launch_tokens(const GateUpArgs &u, const DownArgs &d, int max_hits, cudaStream_t st) {
-    if (d.T <= 8) return launch_layer<T, FMT, G, 1>(u, d, max_hits, st);
-    return launch_layer<T, FMT, G, 2>(u, d, max_hits, st);
+
+template <typename T, int FMT, int G, int NT> int launch_batch(const LayerArgs &a, cudaStream_t st) {
+    constexpr int S = FMT == kWInt4 ? 5 : FMT == kW16 ? 2 : 4, D = FMT == kWInt4 ? 5 : FMT == kW16 ? 2 : 4;
+    const unsigned hits = (unsigned) imin(a.E, a.T * a.k), splits = kScaledX<FMT> ? (unsigned) cdiv(a.T * cdiv(a.H, kKB), 32) : 0u;
+    const int cols = (int) imin(a.T, NT * 8);
+    PTB_EARLY("moe_list_kernel", (moe_list_kernel<T, FMT>), dim3(1 + splits), 1024, 0, st, a.ids, a.probs, a.T, a.k, a.E, a.lists, (const T *) a.x, a.ldx, a.H, a.xs);
+    using U = Walk<FMT, 128, 8, 1>;
+    PTB_EARLY("moe_gate_up_kernel", (moe_gate_up_kernel<T, FMT, G, NT, S>),
+              dim3((unsigned) (kScaledX<FMT> ? cdiv(a.I, kKB) * 2 : cdiv(a.I, kChannels)), hits), U::kThreads, (U::template smem<NT>(S, 1, cols)), st, a); // h's planes are whole blocks
+    using W = Walk<FMT, 64, 8, 1>;
+    PTB_EARLY("moe_down_kernel", (moe_down_kernel<T, FMT, G, NT, D>), dim3((unsigned) cdiv(a.H, W::kRows), hits), W::kThreads,
+              (W::template smem<NT>(D, kScaledX<FMT> ? kHScaled<T> : 2, cols)), st, a);
+    PTB_EARLY("moe_merge_kernel", moe_merge_kernel<T>, dim3((unsigned) cdiv(a.H, 1024), (unsigned) a.T), 128, 0, st, a);
+    return 0;
 }
 
-template <typename T> int launch_format(int format, int group, const GateUpArgs &u, const DownArgs &d, int max_hits, cudaStream_t st) {
+template <typename T, int FMT, int G> int launch_layer(const LayerArgs &a, cudaStream_t st) {
+    int up = 0, down = 0;
+    if (fits_token<T, FMT, G>(a, up, down)) return launch_token<T, FMT, G>(a, up, down, st);
+    if (a.T <= 8) return launch_batch<T, FMT, G, 1>(a, st);
+    return a.T <= 16 ? launch_batch<T, FMT, G, 2>(a, st) : launch_batch<T, FMT, G, 4>(a, st);
+}
+
+template <typename T> int launch_format(int format, int group, const LayerArgs &a, cudaStream_t st) {
     switch (format) {
-    case PTB_E4M3: return launch_tokens<T, kWE4M3, 128>(u, d, max_hits, st);
-    case PTB_E5M2: return launch_tokens<T, kWE5M2, 128>(u, d, max_hits, st);
+    case PTB_E4M3: return launch_layer<T, kWE4M3, 128>(a, st);
+    case PTB_E5M2: return launch_layer<T, kWE5M2, 128>(a, st);
     case PTB_INT4:
-        if (group == 32) return launch_tokens<T, kWInt4, 32>(u, d, max_hits, st);
-        if (group == 64) return launch_tokens<T, kWInt4, 64>(u, d, max_hits, st);
-        return launch_tokens<T, kWInt4, 128>(u, d, max_hits, st);
-    default: return launch_tokens<T, kW16, 128>(u, d, max_hits, st);
+        if (group == 32) return launch_layer<T, kWInt4, 32>(a, st);
+        if (group == 64) return launch_layer<T, kWInt4, 64>(a, st);
+        return launch_layer<T, kWInt4, 128>(a, st);
+    default: return launch_layer<T, kW16, 128>(a, st);
     }
+}
+
+// The workspace's pieces, one after the other; whichever form runs, there is room for it.
+struct Pieces {
+    int64_t xs, hs, rows, lists, total;
+};
+Pieces pieces(int format, int dtype, int64_t T, int64_t k, int64_t H, int64_t I) {
+    auto up = [](int64_t n) { return (n + 15) / 16 * 16; };
+    const bool scaled = format == PTB_E4M3 || format == PTB_E5M2 || format == PTB_INT4;
+    Pieces p{};
+    p.hs    = scaled ? up(scaled_bytes(1, T, H, 128)) : 0;
+    p.rows  = p.hs + up(imax(scaled ? scaled_bytes(dtype == PTB_F16 ? 2 : 1, T * k, I, 64) : 0, T * k * I * 4));
+    p.lists = p.rows + up(T * k * H * 4);
+    p.total = p.lists + list_words(T * k) * 4;
+    return p;
 }
 
 // One weight's description from the arguments of the C call.
@@ -393,6 +569,8 @@ int describe(const char *who, const PtbExpertWeight &p, int format, int64_t rows
 }
 
 } // namespace
+
+int moe_few_status(int *status, int reset) { return few_status(status, reset); }
 } // namespace ptb
 
 using namespace ptb;
@@ -400,9 +578,9 @@ using namespace ptb;
 extern "C" {
 #pragma GCC visibility push(default)
 
-int64_t ptb_moe_few_tokens_workspace(int64_t T, int64_t k, int64_t I) {
-    if (T < 0 || k < 0 || I < 0 || T > kMaxTokens || T * k > kMaxPairs) return -1;
-    return T * k * I * 4 + (list_words(T * k) * 4 + 15) / 16 * 16;
+int64_t ptb_moe_few_tokens_workspace(int dtype, int64_t T, int64_t H, int64_t I, int64_t k, int format) {
+    if (T < 0 || k < 0 || H < 0 || I < 0 || T > kMaxTokens || T * k > kMaxPairs) return -1;
+    return pieces(format, dtype, T, k, H, I).total;
 }
 
 int ptb_moe_few_tokens(const void *x, int dtype, int64_t ldx, int64_t T, int64_t H, int64_t I, int64_t E, const int64_t *ids, const float *probs,
@@ -422,21 +600,22 @@ int ptb_moe_few_tokens(const void *x, int dtype, int64_t ldx, int64_t T, int64_t
     PTB_REQUIRE(x && ids && probs && gate_up && down && workspace && out, PTB_ERR_ARG, "moe_few_tokens: null pointer");
     PTB_REQUIRE(aligned16(x) && aligned16(workspace), PTB_ERR_ALIGN, "moe_few_tokens: x and the workspace must be 16-byte aligned");
     PTB_REQUIRE(format != PTB_INT4 || gate_up->group == down->group, PTB_ERR_ARG, "moe_few_tokens: both weights must have the same group size");
-    GateUpArgs u{};
-    DownArgs d{};
-    if (int rc = describe("the gate and up weight", *gate_up, format, 2 * I, H, u.w)) return rc;
-    if (int rc = describe("the down weight", *down, format, H, I, d.w)) return rc;
+    LayerArgs a{};
+    if (int rc = describe("the gate and up weight", *gate_up, format, 2 * I, H, a.w1)) return rc;
+    if (int rc = describe("the down weight", *down, format, H, I, a.w2)) return rc;
     const int64_t pairs = T * k;
-    __nv_bfloat16 *h = (__nv_bfloat16 *) workspace;
-    const Lists lists = lists_at(h + 2 * pairs * I, pairs);
-    u.x = x; u.ldx = ldx; u.H = (int) H; u.I = (int) I; u.lists = lists; u.h_hi = h; u.h_lo = h + pairs * I;
-    d.T = (int) T; d.H = (int) H; d.I = (int) I; d.lists = lists; d.h_hi = u.h_hi; d.h_lo = u.h_lo; d.out = out;
-    cudaStream_t st = (cudaStream_t) stream;
-    PTB_CUDA(launch_after(moe_list_kernel, dim3(1), 1024, 0, st, 1, ids, probs, (int) T, (int) k, (int) E, lists));
-    PTB_LAUNCH_CHECK("moe_list_kernel");
-    const int max_hits = (int) imin(E, pairs);
-    if (dtype == PTB_BF16) return launch_format<__nv_bfloat16>(format, gate_up->group, u, d, max_hits, st);
-    return launch_format<__half>(format, gate_up->group, u, d, max_hits, st);
+    a.x = x; a.ldx = ldx; a.T = (int) T; a.k = (int) k; a.E = (int) E; a.H = (int) H; a.I = (int) I; a.ids = ids; a.probs = probs; a.out = out;
+    const Pieces at = pieces(format, dtype, T, k, H, I);
+    uint8_t *ws = (uint8_t *) workspace;
+    a.xs    = scaled_rows_at(ws + at.xs, 1, T, H);
+    a.hs    = scaled_rows_at(ws + at.hs, dtype == PTB_F16 ? 2 : 1, pairs, I);
+    a.h32   = (float *) (ws + at.hs);
+    a.h_hi  = (__nv_bfloat16 *) (ws + at.hs);
+    a.h_lo  = a.h_hi + pairs * I;
+    a.rows  = (float *) (ws + at.rows);
+    a.lists = lists_at(ws + at.lists, pairs);
+    if (dtype == PTB_BF16) return launch_format<__nv_bfloat16>(format, gate_up->group, a, (cudaStream_t) stream);
+    return launch_format<__half>(format, gate_up->group, a, (cudaStream_t) stream);
 }
 
 #pragma GCC visibility pop

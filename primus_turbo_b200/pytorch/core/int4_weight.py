@@ -16,9 +16,6 @@ INT4_GROUP_SIZES = (32, 64, 128)
 INT4_BLOCK = 128  # values per block of the packed layout
 INT4_BLOCK_BYTES = INT4_BLOCK // 2
 
-# byte b of a 32-bit word holds value _LOW[b] of its eight in the low nibble and _HIGH[b] in the high one
-_LOW, _HIGH = (0, 4, 1, 5), (2, 6, 3, 7)
-
 
 def _packed_bytes(k: int) -> int:
     return (k + INT4_BLOCK - 1) // INT4_BLOCK * INT4_BLOCK_BYTES
@@ -77,26 +74,18 @@ class Int4Weight:
         assert k % 8 == 0, f"the row length of a 4-bit weight must be a multiple of 8, got {k}"
         padded = torch.nn.functional.pad(codes, (0, -k % INT4_BLOCK)) if k % INT4_BLOCK else codes
         octets = padded.unflatten(-1, (-1, 4, 4, 8)).transpose(-2, -3)  # [..., block, t, q, 8]
-        low, high = (_pick(octets, at) for at in (_LOW, _HIGH))
-        qdata = (low & 15 | high << 4).flatten(-4).contiguous()
+        qdata = (octets[..., :4] & 15 | octets[..., 4:] << 4).flatten(-4).contiguous()
         return cls(qdata, scale.to(torch.bfloat16).contiguous(), None if zero is None else zero.contiguous(), codes.shape, group_size)
 
     def codes(self) -> torch.Tensor:
         """The codes, one a byte, ``[..., N, K]``."""
         words = self.qdata.unflatten(-1, (-1, 4, 4, 4))  # [..., block, t, q, byte]
-        octets = torch.empty((*words.shape[:-1], 8), dtype=torch.uint8, device=self.device)
-        for b in range(4):
-            octets[..., _LOW[b]] = words[..., b] & 15
-            octets[..., _HIGH[b]] = words[..., b] >> 4
+        octets = torch.cat([words & 15, words >> 4], dim=-1)
         return octets.transpose(-2, -3).flatten(-4)[..., : self.shape[-1]].contiguous()
 
     def __repr__(self) -> str:
         kind = "symmetric" if self.zero is None else "zero points"
         return f"Int4Weight(shape={tuple(self.shape)}, group_size={self.group_size}, {kind}, device={self.device})"
-
-
-def _pick(octets: torch.Tensor, at) -> torch.Tensor:
-    return torch.stack([octets[..., i] for i in at], dim=-1)
 
 
 __all__ = ["Int4Weight", "INT4_GROUP_SIZES"]

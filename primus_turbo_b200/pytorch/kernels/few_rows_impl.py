@@ -97,9 +97,10 @@ def gemm_int4_impl(
     m, k = x.shape
     n = codes.shape[0]
     out = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    ws = torch.empty(_lib.lib.ptb_gemm_int4_workspace(dtype_code(x.dtype), m, k, group_size), dtype=torch.uint8, device=x.device)
     with torch.cuda.device(x.device):
         _lib.call("ptb_gemm_int4", ptr(x), dtype_code(x.dtype), x.stride(0), m, n, k, ptr(codes), ptr(scale), ptr(zero), group_size,
-                  ptr(bias), ptr(out), stream_of(x))
+                  ptr(bias), ptr(ws), ptr(out), stream_of(x))
     return out
 
 
@@ -114,7 +115,7 @@ def moe_few_tokens_impl(
     w1, w2 = _aligned(w1), _aligned(w2)
     (T, H), k, E = x.shape, ids.shape[1], w1.shape[0]
     fmt = PTB_INT4 if group_size else dtype_code(w1.dtype)
-    need = _lib.lib.ptb_moe_few_tokens_workspace(T, k, inter)
+    need = _lib.lib.ptb_moe_few_tokens_workspace(dtype_code(x.dtype), T, H, inter, k, fmt)
     out = torch.empty((T, H), dtype=x.dtype, device=x.device)
     ws = torch.empty(max(need, 0), dtype=torch.uint8, device=x.device)
     a = ExpertWeightArg(ptr(w1), ptr(w1_scale), ptr(w1_zero), granularity, group_size)

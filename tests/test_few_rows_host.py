@@ -39,9 +39,8 @@ def test_packed_layout_is_the_documented_one():
             b, r = divmod(k, 128)
             q, r = divmod(r, 32)
             t, i = divmod(r, 8)
-            nibble = i // 2 + 4 * (i % 2)
-            byte = w.qdata[n, b * 64 + (t * 4 + q) * 4 + nibble // 2].item()
-            assert byte >> 4 * (nibble % 2) & 15 == codes[n, k].item()
+            byte = w.qdata[n, b * 64 + (t * 4 + q) * 4 + i % 4].item()
+            assert byte >> 4 * (i // 4) & 15 == codes[n, k].item()
     used = torch.zeros(2, 384, dtype=torch.uint8)
     used[:, :296] = codes
     assert torch.equal(Int4Weight.from_codes(used, torch.ones(2, 3), group_size=128).qdata, w.qdata)  # codes past the end are 0
@@ -148,9 +147,11 @@ def test_argument_errors_are_codes():
     assert quant(codes=p + 4) == -3 and quant(w=None) == -1 and quant(K=1 << 25) == -5
     deq = lambda codes=p, K=128, g=64, out=p, dt=bf, rows=4: L.ptb_dequant_int4(codes, p, None, rows, K, g, out, dt, None)  # noqa: E731
     assert deq(rows=0) == 0 and deq(codes=None) == -1 and deq(K=4) == -3 and deq(g=0) == -1 and deq(out=p + 2) == -3 and deq(dt=4) == -1
-    gemm = lambda x=p, dt=bf, ld=128, M=2, N=16, K=128, codes=p, g=64: L.ptb_gemm_int4(x, dt, ld, M, N, K, codes, p, None, g, None, p, None)  # noqa: E731
+    gemm = lambda x=p, dt=bf, ld=128, M=2, N=16, K=128, codes=p, g=64, ws=p: L.ptb_gemm_int4(x, dt, ld, M, N, K, codes, p, None, g, None, ws, p, None)  # noqa: E731
     assert gemm(M=0) == 0 and gemm(N=0) == 0 and gemm(K=0) == -1 and gemm(dt=f32) == -1 and gemm(ld=127) == -3 and gemm(ld=120) == -1 and gemm(K=12) == -3
-    assert gemm(x=p + 2) == -3 and gemm(codes=p + 8) == -3 and gemm(g=256) == -1 and gemm(x=None) == -1 and gemm(M=1 << 21) == -5
+    assert gemm(x=p + 2) == -3 and gemm(codes=p + 8) == -3 and gemm(g=256) == -1 and gemm(x=None) == -1 and gemm(M=1 << 21) == -5 and gemm(ws=None) == -1 and gemm(ws=p + 8) == -3
+    need = L.ptb_gemm_int4_workspace
+    assert need(bf, 2, 200, 64) >= 2 * 2 * 256 and need(_lib.PTB_F16, 1, 128, 128) >= 2 * 128 and need(f32, 1, 128, 64) == -1 and need(bf, 1, 128, 16) == -1
 
 
 def test_moe_argument_errors_are_codes():
@@ -166,7 +167,8 @@ def test_moe_argument_errors_are_codes():
     assert call(x=None) == -1 and call(x=p + 2) == -3 and call(ws=p + 8) == -3 and call(ws=None) == -1 and call(a=w(data=None)) == -1 and call(b=w(data=p + 4)) == -3
     assert call(fmt=3, a=w(scale=None)) == -1 and call(fmt=5) == -1 and call(fmt=5, a=w(group=32), b=w(group=64)) == -1
     need = L.ptb_moe_few_tokens_workspace
-    assert need(2, 2, 32) >= 2 * 2 * 32 * 4 + (2 + 4 * 4) * 4 and need(129, 1, 8) == -1 and need(128, 9, 8) == -1 and need(0, 1, 8) >= 0
+    assert need(bf, 2, 64, 32, 2, bf) >= 2 * 2 * 32 * 4 and need(bf, 16, 64, 32, 4, 3) >= 64 * (2 * 128 + 64 * 4) + 16 * 2 * 128
+    assert need(bf, 129, 8, 8, 1, bf) == -1 and need(bf, 128, 8, 8, 9, bf) == -1 and need(bf, 0, 8, 8, 1, bf) >= 0
 
 
 # ---- tracing ------------------------------------------------------------------------------------------------------------

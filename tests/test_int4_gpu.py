@@ -110,6 +110,11 @@ def assert_product(y, x, q, bias=None):
     # a product passes through the sums of a group (8), of the blocks of a warp (K / 1024 + 1), of the warps and halves (20) and the bias, each
     # within 2^-23 (the MMA may cut where it does not round) of a partial sum; then one rounding to the output
     k = x.shape[-1]
+    s = spread(q.scale, q.group_size, k).double()
+    # a group's sum is that of bare codes, up to 15, from which zero (up to 15) times the sum of x is taken: 12 operations on sums of that size
+    size = size + xd.abs() @ s.T * (30 * 12 / (k / 1024 + 31))
+    # x is a 16-bit integer in units of at most 2^-14 of the largest of its 128: off by up to half of one
+    size = size + xd.abs().amax(1, keepdim=True) * w.abs().sum(1) * (2.0**8 / (k / 1024 + 31))
     tol = size * (k / 1024 + 31) * 2.0**-23 + want.abs() * torch.finfo(y.dtype).eps / 2 + torch.finfo(y.dtype).smallest_normal * torch.finfo(y.dtype).eps
     assert bool(((y.double() - want).abs() <= tol).all()), ((y.double() - want).abs() / tol).max()
 
@@ -198,7 +203,9 @@ def test_offsets_past_32_bits():
     q = quantize_int4(torch.zeros(1, k, device=DEV, dtype=torch.bfloat16), 128)
     codes = q.qdata.repeat(n, 1)
     scale = torch.full((n, k // 128), 1.0, device=DEV, dtype=torch.bfloat16)
-    codes[-1, 0] = 0x98  # the last row's value 0 is 0, value 2 is one
+    last = torch.full((1, k), 8, device=DEV, dtype=torch.uint8)
+    last[0, 2] = 9  # one
+    codes[-1:] = Int4Weight.from_codes(last, scale[:1], group_size=128).qdata
     big = Int4Weight(codes, scale, None, torch.Size((n, k)), 128)
     x = torch.zeros(1, k, device=DEV, dtype=torch.bfloat16)
     x[0, 2] = 3.0
@@ -207,4 +214,4 @@ def test_offsets_past_32_bits():
     v = dequantize_int4(big)
     assert v[-1, 2] == 1.0 and v[-1].sum() == 1.0
     again = quantize_int4(v, 128)
-    assert torch.equal(again.codes()[-1, :4].cpu(), torch.tensor([8, 8, 15, 8], dtype=torch.uint8)) and bool((again.qdata[:-1] == 0x88).all())
+    assert torch.equal(again.codes()[-1, :4].cpu(), torch.tensor([8, 8, 15, 8], dtype=torch.uint8)) and bool((again.qdata[:-1] == q.qdata).all())

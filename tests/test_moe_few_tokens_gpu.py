@@ -27,14 +27,19 @@ def kept(w, fmt):
         q = quantize_int4(w, int(fmt[5:]) if fmt != "int4_zeros" else 64, symmetric=fmt != "int4_zeros")
         k = w.shape[-1]
         z = 8.0 if q.zero is None else q.zero.double().repeat_interleave(q.group_size, -1)[..., :k]
-        return q, (q.codes().double() - z) * q.scale.double().repeat_interleave(q.group_size, -1)[..., :k]
+        s = q.scale.double().repeat_interleave(q.group_size, -1)[..., :k]
+        v = (q.codes().double() - z) * s
+        v.steps = s
+        return q, v
     gran = {"tensor": G.TENSORWISE, "row": G.ROWWISE, "block": G.BLOCKWISE, "e5m2": G.BLOCKWISE}[fmt]
     cfg = Float8QuantConfig(granularity=gran, block_size=128 if gran == G.BLOCKWISE else None)
     q, _ = create_quantized_weight(w, torch.float8_e5m2 if fmt == "e5m2" else torch.float8_e4m3fn, cfg)
     s = q.scale_inv.double()
     if gran == G.BLOCKWISE:
         s = s.repeat_interleave(128, 1)[:, : w.shape[1]].repeat_interleave(128, 2)[:, :, : w.shape[2]]
-    return q, q.qdata.double() * s
+    v = q.qdata.double() * s
+    v.steps = None
+    return q, v
 
 
 def layer(E, H, I, fmt, dtype=torch.bfloat16, seed=0):
@@ -42,6 +47,17 @@ def layer(E, H, I, fmt, dtype=torch.bfloat16, seed=0):
     w1 = (torch.randn(E, 2 * I, H, generator=g, device=DEV) * H**-0.5).to(dtype)
     w2 = (torch.randn(E, H, I, generator=g, device=DEV) * I**-0.5).to(dtype)
     return kept(w1, fmt), kept(w2, fmt)
+
+
+def detour(v, e, x):
+    """What 4-bit weights add: x is a 16-bit integer in units of at most 2^-14 of the largest of its block, off by up to half of one; bare
+    codes, up to 15, are added up, and zero (up to 15) times the sum of x is taken off: at most 24 operations on sums of that size.  With
+    FP8 weights x is fp16, which holds values below 2^-27 of the largest less exactly."""
+    if not hasattr(v, "steps"):
+        return 0.0
+    if v.steps is None:
+        return v[e].abs().sum(1) * x.abs().max() * 2.0**-37
+    return v.steps[e] @ x.abs() * (30 * 24 * 2.0**-23) + v[e].abs().sum(1) * x.abs().max() * 2.0**-15
 
 
 def reference(x, ids, probs, v1, v2):
@@ -57,15 +73,16 @@ def reference(x, ids, probs, v1, v2):
                 continue
             xd, p = x[t].double(), probs[t, j].double()
             u, size = v1[e] @ xd, v1[e].abs() @ xd.abs()
-            du = size * (H / 1024 + 30) * add  # a term passes through the sums of a scale, of a warp's blocks and of the warps
+            du = size * (H / 1024 + 30) * add + detour(v1, e, xd)  # a term passes through the sums of a scale, of a warp's blocks and of the warps
             a, b = u[:I], u[I:]
             s = torch.sigmoid(a)
             h = a * s * b
-            # silu's slope is at most 1.1; expf, the division and the products within 8 roundings; two bf16 parts leave 2^-17
-            dh = 1.1 * du[:I] * (b.abs() + du[I:]) + (a * s).abs() * du[I:] + h.abs() * (2.0**-17 + 8 * add)
+            # silu's slope is at most 1.1; expf, the division and the products within 8 roundings; two bf16 parts leave 2^-17,
+            # one fp16 (FP8 weights) 2^-11; what integers (4-bit weights) leave is in detour
+            dh = 1.1 * du[:I] * (b.abs() + du[I:]) + (a * s).abs() * du[I:] + h.abs() * ((2.0**-11 if hasattr(v1, "steps") else 2.0**-17) + 8 * add)
             y[t] += p * (v2[e] @ h)
             # the second product: two MMAs an octet, at worst all of an expert's blocks in one warp, 16 warps, the experts of a token
-            err[t] += p.abs() * (v2[e].abs() @ (dh + h.abs() * (I / 8 + 60) * add))
+            err[t] += p.abs() * (v2[e].abs() @ (dh + h.abs() * (I / 8 + 60) * add) + detour(v2, e, h))
     return y, err + y.abs() * torch.finfo(x.dtype).eps / 2 + torch.finfo(x.dtype).smallest_normal * torch.finfo(x.dtype).eps
 
 

@@ -12,14 +12,28 @@ namespace {
 // The scale is rounded before the codes are chosen, so its rounding costs no accuracy beyond a slightly different grid.  A group that
 // holds a NaN or an infinity gets the scale NaN, so that it shows; a group of zeros the scale 0.
 //
-// One thread takes an octet (16 bytes of a 16-bit weight) and writes its 32-bit word; G / 8 neighbouring lanes share a group.
-// HBM-bound: 2 bytes in and half a byte out for a value.
+// HBM-bound: 2 bytes in and half a byte out for a value.  A thread takes the four octets of a block that go into one 16-byte piece of the
+// layout, four lanes a block: four 16-byte loads at once, one index per 32 values.
+struct Blocks { // block -> row, without a division: for n < 2^31, n / d = mulhi(n, mul) >> shift
+    uint32_t count, per_row, mul, shift;
+};
+inline Blocks blocks_of(int64_t rows, int64_t K) {
+    Blocks b;
+    b.per_row = (uint32_t) cdiv<int64_t>(K, kKB);
+    b.count   = (uint32_t) (rows * b.per_row);
+    b.shift   = 0;
+    while ((1ull << b.shift) < b.per_row) ++b.shift; // 2^shift >= d
+    // mul = ceil(2^(31 + shift) / d) < 2^32, its error times n below 2^31 is less than 1 / d of a unit
+    b.mul   = (uint32_t) (((1ull << (31 + b.shift)) + b.per_row - 1) / b.per_row);
+    return b;
+}
+__device__ __forceinline__ uint32_t row_of(const Blocks &b, uint32_t n) { return (uint32_t) ((uint64_t) n * b.mul >> (31 + b.shift)); }
 
-// rint(w / s) with the quotient correct to the last bit where it matters: next to a half-integer the sign of the exact remainder decides
+// rint(w / s), where the quotient may lie next to a half-integer: the sign of the exact remainder decides
 __device__ __forceinline__ float code_steps(float w, float s, float inv) {
-    float r       = rintf(w * inv);
-    r             = fminf(fmaxf(r, -16.0f), 16.0f);
-    const float d = __fmaf_rn(-r, s, w);   // w - r s, rounded once
+    float r       = inv < INFINITY ? w * inv : __fdiv_rn(w, s); // the inverse of a subnormal scale may overflow
+    r             = rintf(fminf(fmaxf(r, -16.0f), 16.0f));
+    const float d = __fmaf_rn(-r, s, w); // w - r s, rounded once
     const float h = 0.5f * s;
     // |d| == s / 2 is the tie (to even); beyond it the product with the inverse was a rounding off
     if (fabsf(d) > h) r += d > 0.0f ? 1.0f : -1.0f;
@@ -27,99 +41,172 @@ __device__ __forceinline__ float code_steps(float w, float s, float inv) {
     return r;
 }
 
+template <typename T> struct Pair; // two 16-bit values
+template <> struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
+template <> struct Pair<__half> { using type = __half2; };
+
 template <typename T, int G, bool kZeros>
-__global__ void __launch_bounds__(256) int4_quant_kernel(const T *w, int64_t octets_per_row, int64_t total, int K, uint32_t *codes,
-                                                          __nv_bfloat16 *scale, uint8_t *zero) {
+__global__ void __launch_bounds__(256) int4_quant_kernel(const T *w, const Blocks blocks, int K, uint4 *codes, __nv_bfloat16 *scale, uint8_t *zero) {
     grid_dep_begin();
-    // thread -> octet of a padded row (a multiple of 16 octets): the lanes of a group are neighbours in a warp
-    const int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x;
-    const bool here = i < total;
-    const int64_t row = here ? i / octets_per_row : 0;
-    const int o = here ? (int) (i - row * octets_per_row) : 0;
-    const int k = o * 8;
-    float v[8];
+    const uint32_t n = blockIdx.x * 64 + (threadIdx.x >> 2);
+    const bool here  = n < blocks.count;
+    const int t      = threadIdx.x & 3;
+    const uint32_t row = here ? row_of(blocks, n) : 0;
+    const int k0       = here ? (int) (n - row * blocks.per_row) * kKB + 8 * t : K;
+    const T *p         = w + (int64_t) row * K + k0;
+    constexpr int kGroups = kKB / G, kPer = 4 / kGroups; // groups of the block, octets of the lane a group
+    float lo[kGroups], hi[kGroups]; // of min(w, 0) and max(w, 0), or hi of |w|; NaN where there is one
+    uint4 u[4][sizeof(T) / 2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-    if (here && k < K) {
-        const T *p = w + row * K + k;
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int i = 0; i < (int) sizeof(T) / 2; ++i) {
+            u[q][i] = make_uint4(0, 0, 0, 0);
+            if (k0 + 32 * q < K) u[q][i] = reinterpret_cast<const uint4 *>(p + 32 * q)[i];
+        }
+#pragma unroll
+    for (int f = 0; f < kGroups; ++f) {
+        lo[f] = hi[f] = 0.0f;
         if constexpr (sizeof(T) == 2) {
-            const uint4 u = *reinterpret_cast<const uint4 *>(p);
+            using P = typename Pair<T>::type;
+            P m = __habs2(*reinterpret_cast<const P *>(&u[f * kPer][0])), l = *reinterpret_cast<const P *>(&u[f * kPer][0]);
+            if constexpr (kZeros) m = l;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = to_f32(reinterpret_cast<const T *>(&u)[j]);
+            for (int q = f * kPer; q < f * kPer + kPer; ++q)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const P v = reinterpret_cast<const P *>(&u[q][0])[j];
+                    m         = __hmax2_nan(m, kZeros ? v : __habs2(v));
+                    if constexpr (kZeros) l = __hmin2_nan(l, v);
+                }
+            const float m0 = to_f32(m.x), m1 = to_f32(m.y), l0 = to_f32(l.x), l1 = to_f32(l.y);
+            hi[f] = m0 != m0 || m1 != m1 ? NAN : fmaxf(fmaxf(m0, m1), 0.0f);
+            if constexpr (kZeros) lo[f] = fminf(fminf(l0, l1), 0.0f);
         } else {
-            const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+#pragma unroll
+            for (int q = f * kPer; q < f * kPer + kPer; ++q)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float v = reinterpret_cast<const float *>(&u[q][0])[j], m = kZeros ? v : fabsf(v);
+                    hi[f] = v != v || hi[f] != hi[f] ? NAN : fmaxf(hi[f], m);
+                    if constexpr (kZeros) lo[f] = fminf(lo[f], v);
+                }
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            const float h = __shfl_xor_sync(0xffffffffu, hi[f], o);
+            hi[f]         = h != h || hi[f] != hi[f] ? NAN : fmaxf(hi[f], h);
+            if constexpr (kZeros) lo[f] = fminf(lo[f], __shfl_xor_sync(0xffffffffu, lo[f], o));
         }
     }
-    float lo = 0.0f, hi = 0.0f; // of min(w, 0) and max(w, 0)
-    bool finite = true;
+    // Divisions are dear: lane t divides for group t, all lanes get all groups' results.
+    float s[kGroups], inv[kGroups], zf[kGroups];
+    {
+        const int f   = t % kGroups;
+        float h       = hi[0], l = lo[0];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        lo = fminf(lo, v[j]);
-        hi = fmaxf(hi, v[j]);
-        finite = finite && fabsf(v[j]) < INFINITY;
-    }
-    if (!finite) hi = INFINITY;
+        for (int i = 1; i < kGroups; ++i)
+            if (f == i) { h = hi[i]; l = lo[i]; }
+        const float wide = kZeros ? __fsub_rn(__fdiv_rn(h, 15.0f), __fdiv_rn(l, 15.0f)) : __fdiv_rn(h, 7.0f);
+        const bool fine  = h < INFINITY && l > -INFINITY;
+        const float sf   = __bfloat162float(__float2bfloat16_rn(fine ? wide : NAN));
+        const float iv   = sf > 0.0f ? __fdiv_rn(1.0f, sf) : 0.0f;
+        float z          = 8.0f;
+        if (kZeros) z = sf > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(-l, sf)), 0.0f), 15.0f) : 0.0f;
 #pragma unroll
-    for (int m = 1; m < G / 8; m <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, m));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, m));
-    }
-    const float wide = kZeros ? __fsub_rn(__fdiv_rn(hi, 15.0f), __fdiv_rn(lo, 15.0f)) : __fdiv_rn(fmaxf(hi, -lo), 7.0f);
-    const bool fine  = hi < INFINITY;
-    const __nv_bfloat16 sb = fine ? __float2bfloat16_rn(wide) : __float2bfloat16_rn(NAN);
-    const float s = __bfloat162float(sb);
-    int z = 8;
-    if (kZeros) z = fine && s > 0.0f ? (int) fminf(fmaxf(rintf(__fdiv_rn(-lo, s)), 0.0f), 15.0f) : 0;
-    uint32_t word = 0;
-    if (fine && s > 0.0f) {
-        const float inv = __fdiv_rn(1.0f, s);
-        const bool plain = inv < INFINITY; // the inverse of a subnormal scale may overflow
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float steps = plain ? code_steps(v[j], s, inv) : rintf(fminf(fmaxf(__fdiv_rn(v[j], s), -16.0f), 16.0f));
-            const int c       = min(max((int) steps + z, 0), 15);
-            word |= (uint32_t) c << int4_shift(j);
+        for (int i = 0; i < kGroups; ++i) {
+            const int from = (threadIdx.x & 28) + i;
+            s[i]   = __shfl_sync(0xffffffffu, sf, from);
+            inv[i] = __shfl_sync(0xffffffffu, iv, from);
+            zf[i]  = kZeros ? __shfl_sync(0xffffffffu, z, from) : 8.0f;
         }
-    } else {
-        word = 0x11111111u * (uint32_t) z;
     }
     if (!here) return;
-    if (k >= K) word = 0;
-    // octet (q, t) of block b is word t * 4 + q
-    const int64_t b = row * (octets_per_row / 16) + o / 16;
-    codes[b * 16 + (o & 3) * 4 + ((o >> 2) & 3)] = word;
-    const int groups = (K + G - 1) / G, g = k / G;
-    if (o % (G / 8) == 0 && g < groups) {
-        scale[row * groups + g] = sb;
-        if (kZeros) zero[row * groups + g] = (uint8_t) z;
+    uint32_t word[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int f = q / kPer;
+        uint32_t b[8];
+        if (sizeof(T) == 2 && inv[f] < INFINITY) {
+            // w / s of 16-bit numbers is a half-integer or at least 2^-13 from one, and the product with the inverse is within 2^-19 of it:
+            // rounded to a multiple of 2^-16 (next to 192) ties are ties again.  Next to 1.5 * 2^23 it is an integer, in the low bits.
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float r = __fmaf_rn(to_f32(reinterpret_cast<const T *>(&u[q][0])[j]), inv[f], 192.0f) - 192.0f;
+                if constexpr (kZeros) r = fminf(fmaxf(r, -zf[f]), 15.0f - zf[f]);
+                r += kFloatBaseValue;
+                if constexpr (kZeros) r += zf[f];
+                b[j] = __float_as_uint(r);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float r = inv[f] > 0.0f ? code_steps(to_f32(reinterpret_cast<const T *>(&u[q][0])[j]), s[f], inv[f]) : 0.0f;
+                b[j]          = (uint32_t) (int) fminf(fmaxf(r + zf[f], 0.0f), 15.0f) ^ (kZeros ? 0u : 8u);
+            }
+        }
+        const uint32_t low = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+        const uint32_t high = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
+        word[q] = (low & 0x0f0f0f0fu) | (high << 4 & 0xf0f0f0f0u);
+        if (!kZeros) word[q] ^= 0x88888888u; // -8 .. 7 in four bits, plus 8
+        if (!(s[f] > 0.0f)) word[q] = 0x11111111u * (uint32_t) zf[f];
+        if (k0 + 32 * q >= K) word[q] = 0;
+    }
+    codes[(int64_t) n * 4 + t] = make_uint4(word[0], word[1], word[2], word[3]);
+    const int groups = (K + G - 1) / G, g = (k0 - 8 * t) / G + t;
+    if (t < kGroups && g < groups) {
+        float sf = s[0], z = zf[0];
+#pragma unroll
+        for (int i = 1; i < kGroups; ++i)
+            if (t == i) { sf = s[i]; z = zf[i]; }
+        scale[(int64_t) row * groups + g] = __float2bfloat16_rn(sf);
+        if constexpr (kZeros) zero[(int64_t) row * groups + g] = (uint8_t) z;
     }
 }
 
 // ---- dequantise --------------------------------------------------------------------------------------------------------
+// The other way, by the same threads.  In bf16 the difference of two codes is exact and its product with the scale is rounded once; in the
+// other types the product is 32-bit (and exact) before it is rounded.
 template <typename T>
-__global__ void __launch_bounds__(256) int4_dequant_kernel(const uint32_t *codes, const __nv_bfloat16 *scale, const uint8_t *zero, int G,
-                                                            int64_t octets_per_row, int64_t total, int K, T *out) {
+__global__ void __launch_bounds__(256) int4_dequant_kernel(const uint4 *codes, const __nv_bfloat16 *scale, const uint8_t *zero, int log_group, const Blocks blocks, int K, T *out) {
     grid_dep_begin();
-    const int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x;
-    if (i >= total) return;
-    const int64_t row = i / octets_per_row;
-    const int o = (int) (i - row * octets_per_row), k = o * 8;
-    if (k >= K) return;
-    const int groups = (K + G - 1) / G;
-    const int64_t at = row * groups + k / G;
-    const float s = __bfloat162float(scale[at]);
-    const int z   = zero != nullptr ? zero[at] : 8;
-    const uint32_t word = codes[(row * (octets_per_row / 16) + o / 16) * 16 + (o & 3) * 4 + ((o >> 2) & 3)];
-    T r[8];
+    const uint32_t n = blockIdx.x * 64 + (threadIdx.x >> 2);
+    if (n >= blocks.count) return;
+    const int t        = threadIdx.x & 3;
+    const uint32_t row = row_of(blocks, n);
+    const int k0       = (int) (n - row * blocks.per_row) * kKB, groups = (K + (1 << log_group) - 1) >> log_group;
+    const uint4 c      = codes[(int64_t) n * 4 + t];
+    const uint32_t word[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r[j] = from_f32<T>((float) ((int) (word >> int4_shift(j) & 15) - z) * s);
-    uint4 u[sizeof(T) / 2];
-    memcpy(u, r, sizeof(r));
-    uint4 *p = reinterpret_cast<uint4 *>(out + row * K + k);
+    for (int q = 0; q < 4; ++q) {
+        const int k = k0 + 32 * q + 8 * t;
+        if (k >= K) continue;
+        const int64_t at = (int64_t) row * groups + ((k0 + 32 * q) >> log_group);
+        const uint32_t z = zero != nullptr ? zero[at] : 8;
+        uint4 *to        = reinterpret_cast<uint4 *>(out + (int64_t) row * K + k);
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            const __nv_bfloat16 s = scale[at];
+            const __nv_bfloat162 s2{s, s};
+            const uint32_t base = 0x43004300u + z * 0x00010001u; // 128 + zero
+            uint32_t p[4]; // codes 0 2, 1 3, 4 6, 5 7
 #pragma unroll
-    for (int j = 0; j < (int) sizeof(T) / 2; ++j) p[j] = u[j];
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t v = (word[q] >> ((i & 1) * 8 + (i >> 1) * 4) & 0x000f000fu) | 0x43004300u;
+                const __nv_bfloat162 d = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&v), *reinterpret_cast<const __nv_bfloat162 *>(&base)), s2);
+                p[i] = *reinterpret_cast<const uint32_t *>(&d);
+            }
+            to[0] = make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[0], p[1], 0x7632), __byte_perm(p[2], p[3], 0x5410), __byte_perm(p[2], p[3], 0x7632));
+        } else {
+            const float s = __bfloat162float(scale[at]), base = 8388608.0f + (float) z;
+            T r[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r[j] = from_f32<T>((__uint_as_float((word[q] >> int4_shift(j) & 15) | 0x4b000000u) - base) * s);
+            uint4 u[sizeof(T) / 2];
+            memcpy(u, r, sizeof(r));
+#pragma unroll
+            for (int i = 0; i < (int) sizeof(T) / 2; ++i) to[i] = u[i];
+        }
+    }
 }
 
 // ---- product of a few rows ----------------------------------------------------------------------------------------------
@@ -272,16 +359,16 @@ int ptb_quant_int4(const void *w, int dtype, int64_t rows, int64_t K, int64_t gr
     if (rows == 0 || K == 0) return 0;
     PTB_REQUIRE(w && codes && scale, PTB_ERR_ARG, "quant_int4: null pointer");
     PTB_REQUIRE(aligned16(w) && aligned16(codes), PTB_ERR_ALIGN, "quant_int4: the weight and the codes must be 16-byte aligned");
-    const int64_t octets = cdiv<int64_t>(K, kKB) * 16, total = rows * octets;
-    PTB_REQUIRE(total <= 256ll * 2147483647ll, PTB_ERR_TOO_LARGE, "quant_int4: too many values");
-    const dim3 grid((unsigned) cdiv<int64_t>(total, 256));
+    PTB_REQUIRE(rows <= 2147483647ll / cdiv<int64_t>(K, kKB), PTB_ERR_TOO_LARGE, "quant_int4: too many values");
+    const Blocks blocks = blocks_of(rows, K);
+    const dim3 grid((unsigned) cdiv<int64_t>(blocks.count, 64));
     PTB_SWITCH_HP(dtype, T, PTB_SWITCH_INT4_GROUP(group, G, {
         if (zero != nullptr)
-            PTB_CUDA(launch_after(int4_quant_kernel<T, G, true>, grid, 256, 0, (cudaStream_t) stream, 1, (const T *) w, octets, total, (int) K,
-                                  (uint32_t *) codes, (__nv_bfloat16 *) scale, (uint8_t *) zero));
+            PTB_CUDA(launch_after(int4_quant_kernel<T, G, true>, grid, 256, 0, (cudaStream_t) stream, 1, (const T *) w, blocks, (int) K, (uint4 *) codes,
+                                  (__nv_bfloat16 *) scale, (uint8_t *) zero));
         else
-            PTB_CUDA(launch_after(int4_quant_kernel<T, G, false>, grid, 256, 0, (cudaStream_t) stream, 1, (const T *) w, octets, total, (int) K,
-                                  (uint32_t *) codes, (__nv_bfloat16 *) scale, (uint8_t *) nullptr));
+            PTB_CUDA(launch_after(int4_quant_kernel<T, G, false>, grid, 256, 0, (cudaStream_t) stream, 1, (const T *) w, blocks, (int) K, (uint4 *) codes,
+                                  (__nv_bfloat16 *) scale, (uint8_t *) nullptr));
     }));
     PTB_LAUNCH_CHECK("int4_quant_kernel");
     return 0;
@@ -297,11 +384,12 @@ int ptb_dequant_int4(const void *codes, const void *scale, const void *zero, int
     if (rows == 0 || K == 0) return 0;
     PTB_REQUIRE(codes && scale && out, PTB_ERR_ARG, "dequant_int4: null pointer");
     PTB_REQUIRE(aligned16(codes) && aligned16(out), PTB_ERR_ALIGN, "dequant_int4: the codes and the output must be 16-byte aligned");
-    const int64_t octets = cdiv<int64_t>(K, kKB) * 16, total = rows * octets;
-    PTB_REQUIRE(total <= 256ll * 2147483647ll, PTB_ERR_TOO_LARGE, "dequant_int4: too many values");
-    const dim3 grid((unsigned) cdiv<int64_t>(total, 256));
-    PTB_SWITCH_HP(out_dtype, T, PTB_CUDA(launch_after(int4_dequant_kernel<T>, grid, 256, 0, (cudaStream_t) stream, 1, (const uint32_t *) codes,
-                                                       (const __nv_bfloat16 *) scale, (const uint8_t *) zero, (int) group, octets, total, (int) K, (T *) out)));
+    PTB_REQUIRE(rows <= 2147483647ll / cdiv<int64_t>(K, kKB), PTB_ERR_TOO_LARGE, "dequant_int4: too many values");
+    const Blocks blocks = blocks_of(rows, K);
+    const dim3 grid((unsigned) cdiv<int64_t>(blocks.count, 64));
+    const int log_group = group == 32 ? 5 : group == 64 ? 6 : 7;
+    PTB_SWITCH_HP(out_dtype, T, PTB_CUDA(launch_after(int4_dequant_kernel<T>, grid, 256, 0, (cudaStream_t) stream, 1, (const uint4 *) codes,
+                                                       (const __nv_bfloat16 *) scale, (const uint8_t *) zero, log_group, blocks, (int) K, (T *) out)));
     PTB_LAUNCH_CHECK("int4_dequant_kernel");
     return 0;
 }

@@ -29,6 +29,8 @@
 
 #include "ptb_common.cuh"
 
+#include <cuda.h>
+
 #include <type_traits>
 
 namespace ptb {
@@ -52,15 +54,17 @@ __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.w
 __device__ __forceinline__ void grid_dep_open() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <typename... P, typename... A>
-inline cudaError_t launch_early(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, A &&...args) {
+inline cudaError_t launch_early(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, unsigned cluster, A &&...args) {
     if (smem > 32 * 1024) // 48 KB without asking, with what the kernel has besides
         if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem)) return e;
     cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {cluster, 1, 1};
     cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
-    cfg.attrs = &attr; cfg.numAttrs = 1;
+    cfg.attrs = attr; cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
@@ -72,19 +76,13 @@ inline int sm_count(int *sms) {
 }
 
 // ---- copies -------------------------------------------------------------------------------------------------------------
-// 16 bytes to shared memory past L1; zeros where nothing is there (nothing is read then)
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there = true) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy4(uint32_t dst, const void *src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
-__device__ __forceinline__ void copies_done() { asm volatile("cp.async.commit_group;" ::: "memory"); } // closes a batch
-template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ uint32_t shared_u32(const void *p) { return (uint32_t) __cvta_generic_to_shared(p); }
 __device__ __forceinline__ uint4 read16(uint32_t at) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
     return v;
 }
+__device__ __forceinline__ void zero16(uint32_t at) { asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory"); }
 __device__ __forceinline__ float read4(uint32_t at) {
     float v;
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
@@ -103,6 +101,8 @@ __device__ __forceinline__ uint2 read8u(uint32_t at) {
 
 // ---- bulk copies and the barriers they complete on ---------------------------------------------------------------------------------
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void bar_end(uint32_t bar) { asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void bar_init_fence() {
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -113,6 +113,10 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
 // 16-byte aligned addresses, a multiple of 16 bytes
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void box_copy(uint32_t dst, const CUtensorMap *map, int byte, int row, int slab, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(byte), "r"(row), "r"(slab)
+                 : "memory");
 }
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
@@ -154,6 +158,11 @@ template <typename T> __device__ __forceinline__ void mma_16(float (&c)[4], uint
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// c = a * b
+__device__ __forceinline__ void mma_16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 template <bool kSigned> __device__ __forceinline__ void mma_8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     if constexpr (kSigned)
         asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -176,44 +185,60 @@ __device__ __forceinline__ void block_scale(float largest, int top, float &scale
 constexpr int kTopInt = 14, kTopHalf = 13;
 __device__ __forceinline__ int fixed16(float v) { return max(min(__float2int_rn(v), 32767), -32768); }
 // Where value k of a block stands: among the bytes that go with byte codes (lane t's four octets are 32 neighbouring bytes), and among the
-// fp16 that go with 4-bit weights (an octet in the order 0 2 1 3 4 6 5 7) or 8-bit ones (in the order of k).
+// fp16 of the walk over rows (octet q of the four lanes: 64 neighbouring bytes; with 4-bit weights an octet's order is 0 2 1 3 4 6 5 7).
 __host__ __device__ __forceinline__ int byte_place(int k) { return (k / 8 % 4) * 32 + (k / 32) * 8 + k % 8; }
-template <int FMT> __host__ __device__ __forceinline__ int half_place(int k) { return FMT == kWInt4 ? (k & ~3) | (k & 1) << 1 | (k & 2) >> 1 : k; }
+template <int FMT> __host__ __device__ __forceinline__ int half_place(int k) {
+    return FMT == kWInt4 ? (k & ~3) | (k & 1) << 1 | (k & 2) >> 1 : (k & ~63) | (k & 8) << 2 | (k & 48) >> 1 | (k & 7);
+}
+
+// ---- weights in shared memory ---------------------------------------------------------------------------------------------------
+// A weight travels in chunks of 256 bytes of 16 rows: two boxes of 128 bytes (one to four blocks), which one thread asks for.  (As sixteen bulk copies, a
+// row each, a chunk cost the warp 20 instructions a copy: an FP8 layer took 82 instead of 63 us.)  Past the end of a row a box is filled with zeros.  The
+// 16-byte units of row r lie in the order unit ^ r % 8.  A quarter of a warp reads four units of two rows at once: rows r and r + 4 meet
+// different banks, so lanes 4 g to 4 g + 3 have row g / 2 + 4 (g % 2) of a tile, and the row 8 further on.
+constexpr int kBoxBytes = 16 * 128, kSlotBytes = 2 * kBoxBytes;
+__device__ __forceinline__ int lane_row() {
+    const int g = (threadIdx.x & 31) >> 2;
+    return g >> 1 | (g & 1) << 2;
+}
+__device__ __forceinline__ uint32_t lane_place() { // of unit t of the row
+    const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+    return lane_row() * 128 + (g & 1) * 64 + (t ^ g >> 1) * 16;
+}
+// slabs of `rows` rows; a tile is 16 rows, or 8 rows of each of two neighbouring slabs
+inline int weight_map(CUtensorMap *map, const void *data, int64_t row_bytes, int64_t rows, int64_t slabs, bool two) {
+    typedef CUresult (*Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
+                               CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static Encode encode = nullptr;
+    if (encode == nullptr) {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        PTB_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found));
+        PTB_REQUIRE(found == cudaDriverEntryPointSuccess && p != nullptr, PTB_ERR_DRIVER, "cuTensorMapEncodeTiled is not available in this driver");
+        encode = (Encode) p;
+    }
+    const cuuint64_t dims[3] = {(cuuint64_t) row_bytes, (cuuint64_t) rows, (cuuint64_t) slabs}, strides[2] = {(cuuint64_t) row_bytes, (cuuint64_t) (row_bytes * rows)};
+    const cuuint32_t box[3] = {128, two ? 8u : 16u, two ? 2u : 1u}, steps[3] = {1, 1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(data), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    PTB_REQUIRE(r == CUDA_SUCCESS, PTB_ERR_DRIVER, "cuTensorMapEncodeTiled failed with CUresult %d", (int) r);
+    return 0;
+}
+// Dynamic shared memory from where boxes may lie; kernels ask for kAlign bytes more.
+constexpr int kAlign = 1024;
+__device__ __forceinline__ uint8_t *aligned(uint8_t *smem) { return smem + (-shared_u32(smem) & (kAlign - 1)); }
 
 // ---- one weight row's share of a lane in a block ----------------------------------------------------------------------
 template <int FMT> struct RowPiece {
     static constexpr int kVecs = FMT == kWInt4 ? 1 : FMT == kW16 ? 4 : 2;
     uint4 v[kVecs];
     static constexpr int kBlockBytes = FMT == kWInt4 ? kInt4BlockBytes : FMT == kW16 ? 256 : 128;
-    // at: the lane's first 16 bytes of the block; slot: where they go, the next ones 512 bytes on
-    static __device__ __forceinline__ void copy(uint32_t slot, const uint8_t *at) {
+    // block i of a chunk; at: the lane's place in the slot, `down` bytes on
+    __device__ __forceinline__ void read(uint32_t at, int i, int down) {
+        if constexpr (FMT == kWInt4) v[0] = read16(((at + (i >> 1) * kBoxBytes) ^ (i & 1) * 64) + down);
+        else
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) copy16(slot + i * 512, at + i * 64);
-    }
-    // the same of a row's last block, where 16-bit and 8-bit rows end after `left` values
-    static __device__ __forceinline__ void copy_last(uint32_t slot, const uint8_t *at, int t, int left) {
-        constexpr int kStep = FMT == kW16 ? 32 : 64; // values from piece to piece
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-            const bool there = i * kStep + t * (kStep / 4) < left;
-            copy16(slot + i * 512, there ? at + i * 64 : at, there);
-        }
-    }
-    __device__ __forceinline__ void read(uint32_t slot) {
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i) v[i] = read16(slot + i * 512);
-    }
-    // from rows as they are: `at` is the lane's first 16 bytes, the next ones 64 on
-    __device__ __forceinline__ void read_row(uint32_t at) {
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i) v[i] = read16(at + i * 64);
-    }
-    // zeros past the first `left` values of a block
-    __device__ __forceinline__ void cut(int t, int left) {
-        constexpr int kStep = FMT == kW16 ? 32 : 64;
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i)
-            if (i * kStep + t * (kStep / 4) >= left) v[i] = make_uint4(0, 0, 0, 0);
+            for (int j = 0; j < kVecs; ++j) v[j] = read16(((at + (FMT == kW16 ? j >> 1 : i) * kBoxBytes) ^ (j & 1) * 64) + down);
     }
     // 4-bit: the eight bytes of octet q
     __device__ __forceinline__ void bytes(int q, uint32_t &lo, uint32_t &hi) const {
@@ -243,8 +268,8 @@ template <int FMT> struct RowPiece {
         }
     }
 };
-// -(base + zero) in both halves, base 1024 or 64: fp16 numbers whose last bit is worth 1 or 1 / 16
-__device__ __forceinline__ uint32_t minus_zero(uint32_t z, int base) { return (base == 1024 ? 0xe400u + z : 0xd400u + 16 * z) * 0x00010001u; }
+constexpr int kChunkRow = 256, kWeightSlots = 2; // slots of a warp
+template <int FMT> constexpr int kChunk = kChunkRow / RowPiece<FMT>::kBlockBytes; // blocks
 
 // ---- scales of a weight ---------------------------------------------------------------------------------------------------
 // 16-bit weights have none; 8-bit ones a float per block of 128 (whatever the granularity: a scale per row or tensor is found again
@@ -256,114 +281,112 @@ template <int FMT> struct RowScale { // one row's
     int stride; // of s8, from block to block
     int count;  // of s4 and z4
 };
-// One block's, in registers: asked for a block ahead, as they are stored; what is made of them waits until they are there.
+// One block's, packed as they are stored.  A lane asks for one block of a chunk, a chunk ahead, and the quad that shares the rows passes
+// them round.
 template <int FMT, int G> struct BlockScale {
-    static constexpr int kN = FMT == kWInt4 ? kKB / G : 1;
-    uint16_t s4[kN];
-    uint8_t z4[kN];
-    float s8;
-    // r: the row's scales from block kb on; `last`: there may be fewer than a block's (past the last group x is zero)
-    __device__ __forceinline__ void load(const RowScale<FMT> &r, int kb, bool last) {
+    static constexpr int kN = FMT == kWInt4 ? kKB / G : 1, kWords = FMT == kWInt4 ? (kN + 1) / 2 : 1;
+    uint32_t s[kWords], z;
+    // the row's scales of block kb; zeros where there are none (there x and the codes are zero)
+    __device__ __forceinline__ void load(const RowScale<FMT> &r, int kb, int blocks) {
         if constexpr (FMT == kWInt4) {
+            z = 0;
 #pragma unroll
             for (int i = 0; i < kN; ++i) {
-                const int g = kN > 1 && last ? min(i, r.count - 1 - kb * kN) : i;
-                s4[i] = r.s4[g];
-                z4[i] = 8;
-                if (r.z4 != nullptr) z4[i] = r.z4[g];
+                const int at     = kb * kN + i;
+                const bool there = at < r.count;
+                const uint32_t v = there ? r.s4[at] : 0u;
+                s[i / 2]         = i % 2 ? s[i / 2] | v << 16 : v;
+                z |= (there && r.z4 != nullptr ? (uint32_t) r.z4[at] : 8u) << (8 * i);
             }
         } else if constexpr (FMT != kW16) {
-            s8 = *r.s8;
+            s[0] = kb < blocks ? __float_as_uint(r.s8[(int64_t) kb * r.stride]) : 0u;
         }
     }
-    static __device__ __forceinline__ void advance(RowScale<FMT> &r, int blocks) {
-        if constexpr (FMT == kWInt4) {
-            r.s4 += blocks * kN;
-            if (r.z4 != nullptr) r.z4 += blocks * kN;
-        } else if constexpr (FMT != kW16) {
-            r.s8 += blocks * r.stride;
-        }
+    __device__ __forceinline__ BlockScale from_lane(int lane) const {
+        BlockScale o;
+        if constexpr (FMT != kW16)
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) o.s[i] = __shfl_sync(0xffffffffu, s[i], lane);
+        if constexpr (FMT == kWInt4) o.z = __shfl_sync(0xffffffffu, z, lane);
+        return o;
     }
-    __device__ __forceinline__ float zero(int i) const { return (float) z4[i]; }
-    __device__ __forceinline__ float scale(int i) const { return FMT == kWInt4 ? __uint_as_float((uint32_t) s4[i] << 16) : s8; }
+    __device__ __forceinline__ float scale(int i) const {
+        if constexpr (FMT != kWInt4) return __uint_as_float(s[0]);
+        return __uint_as_float(i % 2 ? s[i / 2] & 0xffff0000u : s[i / 2] << 16);
+    }
+    // -(1024 + zero) and -(64 + zero) in both halves: fp16 numbers whose last bit is worth 1 or 1 / 16
+    __device__ __forceinline__ void minus_zero(int i, uint32_t &za, uint32_t &zb) const {
+        const uint32_t both = __byte_perm(z, 0, 0x4040 | i | i << 8);
+        za = both + 0xe400e400u;
+        zb = both * 16 + 0xd400d400u;
+    }
 };
 
 // ---- one block ------------------------------------------------------------------------------------------------------------
-// acc[i] += the product of the lane's rows g and g + 8 of the block (p) with the i-th eight rows of x, of which `live` are there.
-// kMasked: x has rows of zeros that the weight is not meant for; `mask` names which of the lane's two columns may be added to: zero
-// times a NaN is not zero.
+// acc[i] += the product of the lane's rows g and g + 8 of the block (p) with the i-th eight rows of x, of NT.
 //
 // 8- and 4-bit weights as fp16.  x(i, term, q) gives octet q of row g of a term; scale(i, f, c) the scale of run f (FL = 64 or 128 long) of
 // column 2 t + c.  A sum goes from scale to scale of the weight, then from scale to scale of x.
-template <int FMT, int G, int FL, int NT, int kTerms, bool kMasked, typename X, typename R>
-__device__ __forceinline__ void half_block(float (&acc)[NT][4], int live, const RowPiece<FMT> (&p)[2], const BlockScale<FMT, G> (&s)[2], unsigned mask, X &&x, R &&scale) {
+template <int FMT, int G, int FL, int NT, int kTerms, int kMost, typename X, typename R>
+__device__ __forceinline__ void half_block(float (&acc)[kMost][4], const RowPiece<FMT> (&p)[2], const BlockScale<FMT, G> (&s)[2], bool zeros, X &&x, R &&scale) {
     static_assert(FL == 64 || FL == 128, "an octet of 8-bit weights covers 64 neighbouring k");
     constexpr int kRun = G < FL ? G : FL;
-    float c[NT][4], b[NT][4];
-    uint32_t za[2] = {0, 0}, zb[2] = {0, 0};
+    constexpr bool kBetween = kRun < FL && NT <= 4; // sums over the groups of a run: registers for a multiplication
+    float c[NT][4], b[kBetween ? NT : 1][4];
+    uint32_t za[2] = {0xe408e408u, 0xe408e408u}, zb[2] = {0xd480d480u, 0xd480d480u}; // of zero points of 8
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         const int group = FMT == kWInt4 ? q * 32 / G : 0;
         const bool start = q % (kRun / 32) == 0, end = q % (kRun / 32) == kRun / 32 - 1, first = q % (FL / 32) < kRun / 32, last = q % (FL / 32) == FL / 32 - 1;
-        if (FMT == kWInt4 && q * 32 % G == 0)
+        if (FMT == kWInt4 && q * 32 % G == 0 && zeros)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                za[h] = minus_zero(s[h].z4[group], 1024);
-                zb[h] = minus_zero(s[h].z4[group], 64);
-            }
+            for (int h = 0; h < 2; ++h) s[h].minus_zero(group, za[h], zb[h]);
         uint32_t wa[4], wb[4];
         p[0].halves(q, za[0], zb[0], wa);
         p[1].halves(q, za[1], zb[1], wb);
+        const float w[2] = {s[0].scale(group), s[1].scale(group)};
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-            if (NT > 1 && i >= live) break;
-            if (start) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.0f;
 #pragma unroll
             for (int term = 0; term < kTerms; ++term) {
                 const uint4 u = x(i, term, q);
-                mma_16<__half>(c[i], wa[0], wb[0], wa[1], wb[1], u.x, u.y);
+                if (start && term == 0) mma_16_first(c[i], wa[0], wb[0], wa[1], wb[1], u.x, u.y);
+                else mma_16<__half>(c[i], wa[0], wb[0], wa[1], wb[1], u.x, u.y);
                 mma_16<__half>(c[i], wa[2], wb[2], wa[3], wb[3], u.z, u.w);
             }
         }
         if (!end) continue;
-        const float w[2] = {s[0].scale(group), s[1].scale(group)};
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-            if (NT > 1 && i >= live) break;
+            if constexpr (kBetween) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) b[i][j] = first ? c[i][j] * w[j >> 1] : b[i][j] + c[i][j] * w[j >> 1];
-            if (!last) continue;
+                for (int j = 0; j < 4; ++j) b[i][j] = first ? c[i][j] * w[j >> 1] : b[i][j] + c[i][j] * w[j >> 1];
+                if (!last) continue;
+            }
             const float xs[2] = {scale(i, q / (FL / 32), 0), scale(i, q / (FL / 32), 1)};
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (!kMasked || (mask >> (j & 1) & 1)) acc[i][j] += b[i][j] * xs[j & 1];
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (kBetween) acc[i][j] += b[i][j] * xs[j & 1];
+                else acc[i][j] += c[i][j] * w[j >> 1] * xs[j & 1];
+            }
         }
     }
 }
 
 // 16-bit weights.  x(i, term, q) gives octet q of row g of a term.
-template <typename T, int NT, int kTerms, bool kMasked, typename X>
-__device__ __forceinline__ void word_block(float (&acc)[NT][4], int live, const RowPiece<kW16> &pa, const RowPiece<kW16> &pb, unsigned mask, X &&x) {
-    float c[NT][4] = {};
+template <typename T, int NT, int kTerms, int kMost, typename X>
+__device__ __forceinline__ void word_block(float (&acc)[kMost][4], const RowPiece<kW16> &pa, const RowPiece<kW16> &pb, X &&x) {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-            if (NT > 1 && i >= live) break;
-            float(&d)[4] = kMasked ? c[i] : acc[i];
 #pragma unroll
             for (int term = 0; term < kTerms; ++term) {
                 const uint4 u = x(i, term, q);
-                mma_16<T>(d, pa.v[q].x, pb.v[q].x, pa.v[q].y, pb.v[q].y, u.x, u.y);
-                mma_16<T>(d, pa.v[q].z, pb.v[q].z, pa.v[q].w, pb.v[q].w, u.z, u.w);
+                mma_16<T>(acc[i], pa.v[q].x, pb.v[q].x, pa.v[q].y, pb.v[q].y, u.x, u.y);
+                mma_16<T>(acc[i], pa.v[q].z, pb.v[q].z, pa.v[q].w, pb.v[q].w, u.z, u.w);
             }
         }
-    if constexpr (kMasked)
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (mask >> (j & 1) & 1) acc[i][j] += c[i][j];
 }
 
 __device__ __forceinline__ void split_half(const RowPiece<kW16> &p, RowPiece<kW16> &hi, RowPiece<kW16> &lo) {
@@ -384,203 +407,195 @@ __device__ __forceinline__ void split_half(const RowPiece<kW16> &p, RowPiece<kW1
 }
 
 // ---- the walk over k ----------------------------------------------------------------------------------------------------
-// WR x WK warps: WR neighbouring sets of 16 weight rows, WK shares of the blocks of k (share s takes blocks s, s + WK, ...).  The WR warps
-// of a share use the same blocks of x, which they copy together; the shares do not wait for one another.
+// WR warps, each with 16 weight rows and two slots of chunks of its own, which it fills again as soon as it has read them.  x is shared: a
+// ring of two pairs of blocks.  A warp that has read a pair says so, and goes on; once it has read the first block of the next, one warp, each in its turn,
+// waits for all to have said so and copies the pair after that there.
 //
-// In shared memory, per share and stage: kTerms * cols rows of 256 bytes of x, for scaled x the runs' scales [cols][128 / FL], then per
-// warp 2 * kVecs * 512 bytes of weights.
-template <int FMT, int FL, int WR, int WK> struct Walk {
-    static constexpr int kThreads = 32 * WR * WK, kRows = 16 * WR; // of weight, per CTA
-    static constexpr int kWarpBytes = 2 * RowPiece<FMT>::kVecs * 512, kRuns = kKB / FL;
-    __host__ __device__ static constexpr int run_bytes(int cols) { return kScaledX<FMT> ? (cols * kRuns * 4 + 15) / 16 * 16 : 0; }
-    __host__ __device__ static constexpr int stage_bytes(int terms, int cols) { return WR * kWarpBytes + terms * cols * 256 + run_bytes(cols); }
-    // what the CTA's shared memory has to hold: the stages, then the sums of the shares
-    template <int NT> static int smem(int stages, int terms, int cols) {
-        const int a = stages * WK * stage_bytes(terms, cols), b = WK * NT * 8 * (kRows + 1) * 4;
-        return a > b ? a : b;
+// Rows of x are shifted against each other so that a quarter of a warp, two rows at once, meets different banks.  Scaled x is
+// stored with its scales: 256 bytes of a block, then the scales of its runs.
+constexpr int kScaledBlock = 256 + 16, kPair = 2, kXPitch = kPair * 256 + 64;
+template <int FMT, int NT, int WR> struct Walk {
+    static constexpr int kThreads = 32 * WR, kRows = 16 * WR; // rows of the weight
+    static constexpr int kXStep = kScaledX<FMT> ? kScaledBlock : 256;
+    static constexpr int kBars = WR * kWeightSlots + 2 * kPair;
+    static constexpr int kSums = NT * 8 * (kRows + 1) * 4;
+    // what the CTA's shared memory has to hold: the slots and the ring, read past its end by what by_live adds, then the sums and `more`
+    static int smem(int terms, int cols, int more = 0) {
+        const int a = WR * kWeightSlots * kSlotBytes + (2 * terms * cols + (NT > 4 ? 15 : 7)) * kXPitch, b = kSums + more;
+        return (a > b ? a : b) + kAlign;
     }
 };
 
-template <int WR> __device__ __forceinline__ void share_barrier(int share) {
-    if constexpr (WR == 1) __syncwarp();
-    else asm volatile("bar.sync %0, %1;" ::"r"(share + 1), "n"(32 * WR) : "memory"); // barrier 0 is the CTA's
+template <int FMT> struct LaneRows { // the warp's tile in the weight's map, and the scales of rows lane_row() and lane_row() + 8
+    int row, slab;
+    RowScale<FMT> scale[2];
+};
+// n blocks of a tile from block kb on into a slot, by one thread
+template <int FMT> __device__ __forceinline__ void fetch_tile(uint32_t slot, const CUtensorMap *map, int kb, int n, int row, int slab, uint32_t bar) {
+    constexpr int kBytes = RowPiece<FMT>::kBlockBytes;
+    const int boxes = (n * kBytes + 127) / 128;
+    bar_expect(bar, boxes * kBoxBytes);
+    box_copy(slot, map, kb * kBytes, row, slab, bar);
+    if (boxes > 1) box_copy(slot + kBoxBytes, map, kb * kBytes + 128, row, slab, bar);
 }
 
-// src: row[h], scale[h]   first byte and scales of the lane's weight row g + 8 h
-//      x(term, col)       where row `col` of x (of a plane) starts;   runs(col)  its scales
-// K: length of a weight row; 16-bit rows of x end there too, a multiple of 8.
-// Weights are fetched ahead of grid_dep_wait, x after it; then the kernel after this one may start (grid_dep_open).
-// A block is few instructions' work, so the pointers of everything a lane copies are kept and moved on by constants.
-template <typename T, int FMT, int G, int FL, int NT, int WR, int WK, int kStages, int kTerms, bool kSplit, typename Src>
-__device__ __forceinline__ void few_rows_walk(float (&acc)[NT][4], uint8_t *smem, int K, int cols, int live, const Src &src) {
-    using W = Walk<FMT, FL, WR, WK>;
-    using Piece = RowPiece<FMT>;
-    constexpr int kRowBytes = Piece::kVecs * 512, kStep = 2 * WR; // rows of x a share copies at a time
-    constexpr int kXPasses = (kTerms * NT * 8 + kStep - 1) / kStep, kRunPasses = kScaledX<FMT> ? (NT * 8 * W::kRuns + 32 * WR - 1) / (32 * WR) : 0;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int wr = warp % WR, share = warp / WR, blocks = (K + kKB - 1) / kKB;
-    const bool ragged = K % kKB != 0;
-    const int x_rows = kTerms * cols, x_bytes = x_rows * 256, stage_bytes = W::stage_bytes(kTerms, cols);
-    const uint32_t base = shared_u32(smem) + share * kStages * stage_bytes, top = base + kStages * stage_bytes;
-    const uint32_t w_at = x_bytes + W::run_bytes(cols) + wr * W::kWarpBytes + lane * 16;
-    const int mine = blocks > share ? (blocks - share + WK - 1) / WK : 0;
-    // A quarter of a warp reads two rows of x at once: the rows of a pair are shifted against each other so that it meets eight different
-    // 16-byte banks (rows a lane copies are all even or all odd).
-    constexpr int kShift = FMT == kWE4M3 || FMT == kWE5M2 ? 1 : 4;
-    const int unit = lane & 15, x_first = wr * 2 + (lane >> 4), run_first = wr * 32 + lane;
-    const uint32_t x_at = x_first * 256 + (unit ^ (x_first & 1) * kShift) * 16;
+// body(the number of eights of x as a constant, or one more): branches on it in the middle of a block cost ten instructions each.
+template <int NT, typename F> __device__ __forceinline__ void by_live(int live, F &&body) {
+    constexpr int kLess = NT > 4 ? NT - 2 : NT - 1;
+    if constexpr (kLess > 0)
+        if (live <= kLess) return by_live<kLess>(live, body);
+    body(std::integral_constant<int, NT>{});
+}
 
-    const uint8_t *wp[2], *xp[kXPasses];
-    const float *rp[kRunPasses > 0 ? kRunPasses : 1];
-    int kb_w = share, kb_x = share;
-    wp[0] = src.row[0] + (int64_t) share * Piece::kBlockBytes + t * 16;
-    wp[1] = src.row[1] + (int64_t) share * Piece::kBlockBytes + t * 16;
-    auto fetch_weights = [&](uint32_t slot) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (FMT == kWInt4 || !ragged || kb_w != blocks - 1) Piece::copy(slot + w_at + h * kRowBytes, wp[h]);
-            else Piece::copy_last(slot + w_at + h * kRowBytes, wp[h], t, K - kb_w * kKB);
-            wp[h] += WK * Piece::kBlockBytes;
-        }
-        kb_w += WK;
+// src: a LaneRows, and x(term, col): where row `col` of x (of a plane) starts.  [begin, end): blocks of k, begin at the start of a chunk.
+// K: length of a weight row; 16-bit rows of x end there too.
+// Weights are fetched ahead of grid_dep_wait, x after it; then the kernel after this one may start (grid_dep_open).
+// Called by all threads; what the shared memory held is read, and the barriers are free again, when it returns.
+template <typename T, int FMT, int G, int FL, int NT, int WR, int kTerms, bool kSplit, typename Src>
+__device__ __forceinline__ void few_rows_walk(float (&acc)[NT][4], uint8_t *smem, uint64_t *bars, const CUtensorMap *map, int K, int cols, int begin, int end, const Src &src) {
+    using W = Walk<FMT, NT, WR>;
+    using Piece = RowPiece<FMT>;
+    constexpr int CB = kChunk<FMT>, kXPasses = (kTerms * NT * 8 + 31) / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int blocks = (K + kKB - 1) / kKB, live = (cols + 7) / 8, x_rows = kTerms * cols;
+    const uint32_t ring = shared_u32(smem) + warp * (kWeightSlots * kSlotBytes), x_ring = shared_u32(smem) + WR * (kWeightSlots * kSlotBytes), x_stage = x_rows * kXPitch;
+    const uint32_t w_bars = shared_u32(bars) + warp * (kWeightSlots * 8), x_bars = shared_u32(bars) + WR * (kWeightSlots * 8), read_bars = x_bars + 2 * 8;
+    if (threadIdx.x < W::kBars) bar_init(shared_u32(bars) + threadIdx.x * 8, threadIdx.x < W::kBars - 2 ? 1 : WR);
+    bar_init_fence();
+    __syncthreads();
+
+    int kb_w = begin;
+    auto fetch_weights = [&](int slot) {
+        if (kb_w < end && lane == 0) fetch_tile<FMT>(ring + slot * kSlotBytes, map, kb_w, min(CB, end - kb_w), src.row, src.slab, w_bars + slot * 8);
+        kb_w += CB;
     };
-    auto fetch_x = [&](uint32_t slot) {
+    BlockScale<FMT, G> next[2], mine[2];
 #pragma unroll
-        for (int i = 0; i < kXPasses; ++i)
-            if (x_first + i * kStep < x_rows) {
-                copy16(slot + x_at + i * (kStep * 256), xp[i], kScaledX<FMT> || !ragged || kb_x * kKB + unit * 8 < K);
-                xp[i] += WK * 256;
-            }
+    for (int h = 0; h < 2; ++h) next[h].load(src.scale[h], begin + t, CB > 1 || t == 0 ? end : 0);
 #pragma unroll
-        for (int i = 0; i < kRunPasses; ++i)
-            if (run_first + i * 32 * WR < cols * W::kRuns) {
-                copy4(slot + x_bytes + (run_first + i * 32 * WR) * 4, rp[i]);
-                rp[i] += WK * W::kRuns;
-            }
-        kb_x += WK;
-    };
-    BlockScale<FMT, G> s[2], next[2];
-    RowScale<FMT> sp[2] = {src.scale[0], src.scale[1]};
-    int kb_s = share;
-    auto load_scales = [&] {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            next[h].load(sp[h], kb_s, kb_s == blocks - 1);
-            BlockScale<FMT, G>::advance(sp[h], WK);
-        }
-        kb_s += WK;
-    };
-    if (mine > 0) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) BlockScale<FMT, G>::advance(sp[h], share);
-        load_scales();
-    }
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i)
-        if (i < mine) fetch_weights(base + i * stage_bytes);
+    for (int i = 0; i < kWeightSlots; ++i) fetch_weights(i);
     grid_dep_wait();
     grid_dep_open();
+    const uint8_t *xp[kXPasses];
 #pragma unroll
     for (int i = 0; i < kXPasses; ++i) {
-        const int row = min(x_first + i * kStep, x_rows - 1), term = kTerms > 1 && row >= cols ? 1 : 0;
-        xp[i] = src.x(term, row - term * cols) + (int64_t) share * 256 + unit * 16;
+        const int row = min(lane + 32 * i, x_rows - 1), term = kTerms > 1 && row >= cols ? 1 : 0;
+        xp[i] = src.x(term, row - term * cols);
     }
-#pragma unroll
-    for (int i = 0; i < kRunPasses; ++i) {
-        const int at = min(run_first + i * 32 * WR, cols * W::kRuns - 1);
-        rp[i] = src.runs(at / W::kRuns) + share * W::kRuns + at % W::kRuns;
-    }
-    uint32_t fill = base, drain = base;
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) {
-        if (i < mine) fetch_x(fill);
-        copies_done();
-        fill += stage_bytes;
-    }
-    // Where the lane finds its row of the i-th eight of x; a row that is not there reads another, its column is not looked at.
-    uint32_t x_row[NT], x_odd[NT];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        const int col = min(i * 8 + g, cols - 1);
-        x_row[i] = col * 256;
-        x_odd[i] = (col & 1) * kShift * 16;
-    }
-    const uint32_t term_bytes = cols * 256, term_odd = (cols & 1) * kShift * 16;
-    for (int it = 0; it < mine; ++it) {
-        copies_wait<kStages - 2>();
-        share_barrier<WR>(share); // the block is there for every warp, and the stage before it is read by every warp
-        if (it + kStages - 1 < mine) {
-            fetch_weights(fill);
-            fetch_x(fill);
-            fill += stage_bytes;
-            if (fill == top) fill = base;
+    auto fetch_x = [&](int kb, int stage) { // by one warp
+        const int n = min(kPair, end - kb);
+        uint32_t bytes = n * W::kXStep;
+        const uint32_t to = x_ring + stage * x_stage;
+        if (!kScaledX<FMT> && (kb + n) * kKB > K) { // zeros behind the end: the weights are zero there too, but what lies here might be a NaN
+            bytes = (K - kb * kKB) * 2;
+            for (int i = lane; i < x_rows * (kPair * 16); i += 32)
+                if ((i % (kPair * 16)) * 16 >= bytes) zero16(to + i / (kPair * 16) * kXPitch + (i % (kPair * 16)) * 16);
+            __syncwarp();
         }
-        copies_done();
-        s[0] = next[0];
-        s[1] = next[1];
-        if (it + 1 < mine) load_scales();
-        Piece p[2];
-        p[0].read(drain + w_at);
-        p[1].read(drain + w_at + kRowBytes);
-        auto x = [&](int i, int term, int q) {
-            const int at = FMT == kWE4M3 || FMT == kWE5M2 ? 128 * (q / 2) + 32 * t + 16 * (q % 2) : 64 * q + 16 * t;
-            return read16(drain + x_row[i] + term * term_bytes + (at ^ x_odd[i] ^ (term * term_odd)));
-        };
-        if constexpr (kScaledX<FMT>) { // (a column that is not there reads what lies behind the runs)
-            const uint32_t run_at = drain + x_bytes + 2 * t * W::kRuns * 4;
-            half_block<FMT, G, FL, NT, kTerms, false>(acc, live, p, s, 3, x, [&](int i, int f, int c) { return read4(run_at + ((i * 8 + c) * W::kRuns + f) * 4); });
-        } else if constexpr (!kSplit) {
-            word_block<T, NT, kTerms, false>(acc, live, p[0], p[1], 3, x);
-        } else { // fp16 weights become the sum of two bf16, exactly
-            Piece ha, hb, la, lb;
-            split_half(p[0], ha, la);
-            split_half(p[1], hb, lb);
-            word_block<T, NT, kTerms, false>(acc, live, ha, hb, 3, x);
-            word_block<T, NT, 1, false>(acc, live, la, lb, 3, x);
+        if (lane == 0) bar_expect(x_bars + stage * 8, x_rows * bytes);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kXPasses; ++i)
+            if (lane + 32 * i < x_rows) bulk_copy(to + (lane + 32 * i) * kXPitch, xp[i] + (int64_t) kb * W::kXStep, bytes, x_bars + stage * 8);
+    };
+    if (warp < 2 && begin + warp * kPair < end) fetch_x(begin + warp * kPair, warp);
+
+    const uint32_t w_lane = ring + lane_place();
+    const uint32_t x_lane = x_ring + g * kXPitch + t * 16, run_lane = x_ring + 2 * t * kXPitch + 256, term_bytes = cols * kXPitch;
+    int slot = 0, in = 0; // in: blocks done of the chunk
+    uint32_t w_parity = 0, x_at = 0, w_at = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (int kb = begin; kb < end; ++kb) {
+        if (in == 0) {
+            if (ok) ok = __all_sync(0xffffffffu, bar_wait(w_bars + slot * 8, w_parity));
+            w_at = w_lane + slot * kSlotBytes;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                mine[h] = next[h];
+                next[h].load(src.scale[h], kb + CB + t, end);
+            }
         }
-        drain += stage_bytes;
-        if (drain == top) drain = base;
+        const int pair = (kb - begin) / kPair, stage = pair & 1;
+        const bool first = (kb - begin) % kPair == 0;
+        if (first) {
+            if (ok) ok = __all_sync(0xffffffffu, bar_wait(x_bars + stage * 8, pair >> 1 & 1));
+            x_at = stage * x_stage;
+        }
+        if (ok) {
+            Piece p[2];
+            p[0].read(w_at, in, 0);
+            p[1].read(w_at, in, 8 * 128);
+            auto x = [&](int i, int term, int q) { return read16(x_lane + x_at + i * (8 * kXPitch) + term * term_bytes + q * 64); };
+            BlockScale<FMT, G> s[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) s[h] = mine[h].from_lane((lane & 28) | in);
+            by_live<NT>(live, [&](auto n) {
+                constexpr int N = decltype(n)::value;
+                if constexpr (kScaledX<FMT>) {
+                    half_block<FMT, G, FL, N, kTerms>(acc, p, s, src.scale[0].z4 != nullptr, x, [&](int i, int f, int c) { return read4(run_lane + x_at + (i * 8 + c) * kXPitch + f * 4); });
+                } else if constexpr (!kSplit) {
+                    word_block<T, N, kTerms>(acc, p[0], p[1], x);
+                } else { // fp16 weights become the sum of two bf16, exactly
+                    Piece ha, hb, la, lb;
+                    split_half(p[0], ha, la);
+                    split_half(p[1], hb, lb);
+                    word_block<T, N, kTerms>(acc, ha, hb, x);
+                    word_block<T, N, 1>(acc, la, lb, x);
+                }
+            });
+        }
+        if (++in == CB || kb == end - 1) {
+            __syncwarp();
+            if (ok) fetch_weights(slot);
+            in = 0;
+            if (++slot == kWeightSlots) { slot = 0; w_parity ^= 1; }
+        }
+        x_at += W::kXStep;
+        if (!first || kb == end - 1) {
+            __syncwarp();
+            if (lane == 0) bar_arrive(read_bars + stage * 8);
+        }
+        if (first && pair > 0 && kb + kPair < end && warp == pair % WR) {
+            if (ok) ok = __all_sync(0xffffffffu, bar_wait(read_bars + (stage ^ 1) * 8, (pair - 1) >> 1 & 1));
+            if (ok) fetch_x(kb + kPair, stage ^ 1);
+        }
     }
-    copies_wait<0>();
+    if (!ok) { // the result is incomplete; what is on its way lands before the CTA gives its memory back
+        if (lane == 0) atomicExch(&g_few_status, 5);
+        for (int i = 0; i < kWeightSlots; ++i) bar_wait(w_bars + i * 8, i < slot ? w_parity ^ 1 : w_parity);
+        const int last = (end - 1 - begin) / kPair;
+        for (int i = max(last - 1, 0); i <= last; ++i) bar_wait(x_bars + (i & 1) * 8, i >> 1 & 1);
+    }
+    __syncthreads();
+    if (threadIdx.x < W::kBars) bar_end(shared_u32(bars) + threadIdx.x * 8);
 }
 
-// The shares' sums in shared memory [share][column][row]: sum(column, row) adds them up, in the shares' order.
-template <int NT, int WR, int WK> struct ShareSums {
-    static constexpr int kPitch = 16 * WR + 1;
+// The sums in shared memory [column][row].
+template <int FMT, int NT, int WR> struct RowSums {
+    static constexpr int kPitch = Walk<FMT, NT, WR>::kRows + 1;
     float *part;
-    __device__ __forceinline__ ShareSums(const float (&acc)[NT][4], uint8_t *smem) : part(reinterpret_cast<float *>(smem)) {
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-        __syncthreads(); // the stages are read
-        float *mine = part + (warp / WR) * (NT * 8) * kPitch + warp % WR * 16;
+    __device__ __forceinline__ RowSums(const float (&acc)[NT][4], uint8_t *smem) : part(reinterpret_cast<float *>(smem)) {
+        const int warp = threadIdx.x >> 5, t = threadIdx.x & 3;
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) mine[(i * 8 + 2 * t + (j & 1)) * kPitch + g + (j >> 1) * 8] = acc[i][j];
+            for (int j = 0; j < 4; ++j) part[(i * 8 + 2 * t + (j & 1)) * kPitch + warp * 16 + lane_row() + (j >> 1) * 8] = acc[i][j];
         __syncthreads();
     }
-    __device__ __forceinline__ float sum(int column, int row) const {
-        float s = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WK; ++w) s += part[(w * NT * 8 + column) * kPitch + row];
-        return s;
-    }
+    __device__ __forceinline__ float sum(int column, int row) const { return part[column * kPitch + row]; }
 };
 
 // ---- scaling rows of x -------------------------------------------------------------------------------------------------------
-struct ScaledRows { // planes [rows][pitch] of fp16, scales [rows][blocks * 128 / FL]
+struct ScaledRows { // [terms][rows][blocks] of 128 fp16 and, in the first term, the scales of the block's runs
     uint8_t *planes;
-    int64_t plane;  // bytes from plane to plane
-    int64_t pitch;  // bytes of a row
-    float *runs;
-    int blocks;
+    int64_t plane; // bytes from term to term
+    int64_t pitch; // bytes of a row
 };
-inline int64_t scaled_bytes(int terms, int64_t rows, int64_t K, int FL) {
-    const int64_t blocks = cdiv<int64_t>(K, kKB);
-    return rows * blocks * (terms * kKB * 2 + kKB / FL * 4);
-}
-inline ScaledRows scaled_rows_at(void *p, int terms, int64_t rows, int64_t K) {
-    const int64_t blocks = cdiv<int64_t>(K, kKB), pitch = blocks * kKB * 2;
-    return {(uint8_t *) p, rows * pitch, pitch, (float *) ((uint8_t *) p + terms * rows * pitch), (int) blocks};
+inline int64_t scaled_bytes(int terms, int64_t rows, int64_t K) { return terms * rows * cdiv<int64_t>(K, kKB) * kScaledBlock; }
+inline ScaledRows scaled_rows_at(void *p, int64_t rows, int64_t K) {
+    const int64_t pitch = cdiv<int64_t>(K, kKB) * kScaledBlock;
+    return {(uint8_t *) p, rows * pitch, pitch};
 }
 
 // The lane's four neighbouring values of a block of a row, zero past its end.
@@ -597,43 +612,36 @@ template <typename T> __device__ __forceinline__ void load_four(const T *x, int 
         for (int j = 0; j < 4; ++j) v[j] = to_f32(reinterpret_cast<const T *>(&u)[j]);
     }
 }
-__device__ __forceinline__ float largest_of(const float (&v)[4], bool &fine) {
+__device__ __forceinline__ float largest_of(const float (&v)[4]) { // of the warp's finite ones
     float largest = 0.0f;
-    fine = true;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float m = fabsf(v[j]);
-        if (m < INFINITY) largest = fmaxf(largest, m);
-        else fine = false;
-    }
+    for (int j = 0; j < 4; ++j)
+        if (fabsf(v[j]) < INFINITY) largest = fmaxf(largest, fabsf(v[j]));
     return warp_max(largest);
 }
 
-// A warp scales a block, four values a lane, to fp16: `to` is the block's place in the first plane.
-template <int FMT, int kTerms> __device__ __forceinline__ void scale_to_half(const float (&v)[4], uint8_t *to, int64_t plane, float *run) {
-    const int lane = threadIdx.x & 31;
-    bool fine;
-    float scale, inv;
-    block_scale(largest_of(v, fine), kTopHalf, scale, inv);
+// Values k to k + 3 of a block, times inv, as fp16; or what that leaves.
+template <int FMT> __device__ __forceinline__ void put_halves(uint8_t *block, int k, const float (&v)[4], float inv, bool rest) {
+    __half h[4];
 #pragma unroll
-    for (int term = 0; term < kTerms; ++term) {
-        __half h[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float x = v[j] * inv;
-            h[half_place<FMT>(j)] = term == 0 ? __float2half_rn(x) : __float2half_rn(fabsf(x) < INFINITY ? x - __half2float(__float2half_rn(x)) : 0.0f);
-        }
-        uint2 u;
-        memcpy(&u, h, 8);
-        *reinterpret_cast<uint2 *>(to + term * plane + lane * 8) = u;
+    for (int j = 0; j < 4; ++j) {
+        const float s = v[j] * inv;
+        h[half_place<FMT>(j)] = !rest ? __float2half_rn(s) : __float2half_rn(fabsf(s) < INFINITY ? s - __half2float(__float2half_rn(s)) : 0.0f);
     }
-    if (lane == 0) *run = scale;
+    uint2 u;
+    memcpy(&u, h, 8);
+    *reinterpret_cast<uint2 *>(block + (half_place<FMT>(k) & ~3) * 2) = u;
 }
 
+// A warp scales block kb of a row, four values a lane.
 template <typename T, int FMT> __device__ __forceinline__ void scale_block(const T *x, int K, int kb, int64_t row, const ScaledRows &out) {
-    float v[4];
-    load_four(x, K, kb * kKB + (threadIdx.x & 31) * 4, v);
-    scale_to_half<FMT, 1>(v, out.planes + row * out.pitch + kb * (kKB * 2), out.plane, out.runs + row * out.blocks + kb);
+    const int lane = threadIdx.x & 31;
+    float v[4], scale, inv;
+    load_four(x, K, kb * kKB + lane * 4, v);
+    block_scale(largest_of(v), kTopHalf, scale, inv);
+    uint8_t *to = out.planes + row * out.pitch + (int64_t) kb * kScaledBlock;
+    put_halves<FMT>(to, lane * 4, v, inv, false);
+    if (lane == 0) *reinterpret_cast<float *>(to + 256) = scale;
 }
 
 template <typename T, int FMT> __global__ void __launch_bounds__(128) scale_rows_kernel(const T *x, int64_t ldx, int M, int K, const ScaledRows out) {

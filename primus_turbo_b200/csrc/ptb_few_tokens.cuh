@@ -19,10 +19,7 @@
 namespace ptb {
 namespace {
 
-constexpr int kTokenWarps = 16, kTokenStages = 2, kTokenCols = 8;
-constexpr int kChunkRow = 256, kChunkPitch = kChunkRow + 64; // bytes of a row a chunk; rows of a pair read at once lie on different banks
-constexpr int kSlotBytes = 16 * kChunkPitch;
-template <int FMT> constexpr int kChunk = kChunkRow / RowPiece<FMT>::kBlockBytes; // blocks
+constexpr int kTokenWarps = 16, kTokenCols = 8;
 
 // x in shared memory: per block kTerms x cols rows (and once more, zeros), then per block and column the scales (and sums).
 template <int FMT, int G> struct TokenX {
@@ -32,7 +29,7 @@ template <int FMT, int G> struct TokenX {
     __host__ __device__ static constexpr int run_bytes(int cols) { return cols * kRuns * 8; }
     __host__ __device__ static constexpr int bytes(int terms, int cols, int blocks) { return (blocks + 1) * block_bytes(terms, cols) + blocks * run_bytes(cols); }
 };
-inline int token_smem(int x_bytes, int cols) { return kTokenWarps * kTokenStages * kSlotBytes + (x_bytes + 15) / 16 * 16 + kTokenWarps * cols * 17 * 4; }
+inline int token_smem(int x_bytes, int cols) { return kTokenWarps * kWeightSlots * kSlotBytes + (x_bytes + 15) / 16 * 16 + kTokenWarps * cols * 17 * 4 + kAlign; }
 
 // Staging: eight lanes share a block of a column, sixteen neighbouring values (two octets) each; a warp has four blocks at a time.  A CTA runs
 // this once, on cold instruction caches: few instructions count, and few different ones.
@@ -133,59 +130,49 @@ __device__ __forceinline__ void stage_blocks(uint8_t *x, uint8_t *runs, int n, i
         }
 }
 
-// src.open(tile, segment)     from here on `row` (first byte of row lane % 16 of the tile) and scale[h] (of rows lane / 4 + 8 h) are that part's
+// src.open(tile, segment)     from here on row, slab and scale (a LaneRows) are that part's
 // src.mask(segment, column)   with kMasked: whether the segment's weight is meant for the column
 // stage(x, runs)              stages all of x in shared memory (called by all warps, after grid_dep_wait)
 // finish(tile, sum)           called by one warp for each tile; sum(column, row) is there for columns below `cols` and rows below 16
 // 1 << log_shares warps a tile; segments * blocks blocks of k a tile; K: length of a weight row (of a segment).
 // kEarly: weights may be fetched ahead of grid_dep_wait.
 template <typename T, int FMT, int G, int kTerms, bool kSplit, bool kMasked, bool kEarly, typename Src, typename Stage, typename Finish>
-__device__ __forceinline__ void few_tokens_walk(uint8_t *smem, int cols, int tiles, int log_shares, int segments, int K, const Src &src, Stage &&stage, Finish &&finish) {
+__device__ __forceinline__ void few_tokens_walk(uint8_t *smem, const CUtensorMap *map, int cols, int tiles, int log_shares, int segments, int K, const Src &src, Stage &&stage, Finish &&finish) {
     using X = TokenX<FMT, G>;
     using Piece = RowPiece<FMT>;
     constexpr int CB = kChunk<FMT>;
-    __shared__ uint64_t full[kTokenWarps * kTokenStages];
+    __shared__ uint64_t full[kTokenWarps * kWeightSlots];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int blocks = (K + kKB - 1) / kKB, total = segments * blocks;
     const int tile = blockIdx.x * (kTokenWarps >> log_shares) + (warp >> log_shares), share = warp & ((1 << log_shares) - 1);
-    const uint32_t ring = shared_u32(smem) + warp * (kTokenStages * kSlotBytes), bars = shared_u32(full) + warp * (kTokenStages * 8);
-    uint8_t *x0 = smem + kTokenWarps * kTokenStages * kSlotBytes, *runs0 = x0 + (total + 1) * X::block_bytes(kTerms, cols);
+    const uint32_t ring = shared_u32(smem) + warp * (kWeightSlots * kSlotBytes), bars = shared_u32(full) + warp * (kWeightSlots * 8);
+    uint8_t *x0 = smem + kTokenWarps * kWeightSlots * kSlotBytes, *runs0 = x0 + (total + 1) * X::block_bytes(kTerms, cols);
     float *part = reinterpret_cast<float *>(x0 + (X::bytes(kTerms, cols, total) + 15) / 16 * 16);
     const int begin = tile < tiles ? share * total >> log_shares : 0, end = tile < tiles ? (share + 1) * total >> log_shares : 0;
 
-    if (lane < kTokenStages) bar_init(bars + lane * 8, 1);
+    if (lane < kWeightSlots) bar_init(bars + lane * 8, 1);
     bar_init_fence();
     __syncwarp();
     // what is fetched next
     Src ahead = src;
-    const uint8_t *wp = nullptr;
     const int seg0 = segments == 1 ? 0 : begin / blocks, kb0 = begin - seg0 * blocks;
     int left_w = end - begin, seg_w = seg0, kb_w = kb0;
-    auto aim_w = [&] {
-        ahead.open(tile, seg_w);
-        wp = ahead.row + (int64_t) kb_w * Piece::kBlockBytes;
-    };
     auto fetch_chunk = [&](int slot) {
         if (left_w <= 0) return;
         const int n = min(min(CB, blocks - kb_w), left_w);
-        // 8- and 16-bit rows end with their last value
-        const uint32_t bytes = FMT != kWInt4 && kb_w + n == blocks ? (uint32_t) (K - kb_w * kKB) * (Piece::kBlockBytes / kKB) : (uint32_t) n * Piece::kBlockBytes;
-        if (lane == 0) bar_expect(bars + slot * 8, 16 * bytes);
-        __syncwarp();
-        if (lane < 16) bulk_copy(ring + slot * kSlotBytes + lane * kChunkPitch, wp, bytes, bars + slot * 8);
+        if (lane == 0) fetch_tile<FMT>(ring + slot * kSlotBytes, map, kb_w, n, ahead.row, ahead.slab, bars + slot * 8);
         left_w -= n;
         kb_w += n;
-        wp += n * Piece::kBlockBytes;
         if (kb_w == blocks && left_w > 0) {
             kb_w = 0;
             ++seg_w;
-            aim_w();
+            ahead.open(tile, seg_w);
         }
     };
     if constexpr (!kEarly) grid_dep_wait();
-    if (left_w > 0) aim_w();
+    if (left_w > 0) ahead.open(tile, seg_w);
 #pragma unroll 1
-    for (int i = 0; i < kTokenStages; ++i) fetch_chunk(i);
+    for (int i = 0; i < kWeightSlots; ++i) fetch_chunk(i);
     if constexpr (kEarly) grid_dep_wait();
     grid_dep_open();
     for (int i = threadIdx.x * 4; i < X::block_bytes(kTerms, cols); i += 32 * kTokenWarps * 4) *reinterpret_cast<uint32_t *>(x0 + total * X::block_bytes(kTerms, cols) + i) = 0;
@@ -203,7 +190,7 @@ __device__ __forceinline__ void few_tokens_walk(uint8_t *smem, int cols, int til
         token[j] = (2 * t + j) & (tokens - 1);
         place[j] = (2 * t + j) >> shift;
     }
-    const uint32_t w_lane = ring + g * kChunkPitch + t * 16;
+    const uint32_t w_lane = ring + lane_place();
     using Sum = std::conditional_t<FMT == kWInt4, int, float>;
     Sum c[2][4]; // 4-bit: products with high and with low bytes; otherwise two chains of MMAs, each waiting for its last
     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -254,8 +241,8 @@ __device__ __forceinline__ void few_tokens_walk(uint8_t *smem, int cols, int til
         if constexpr (FMT == kWInt4) {
             if (unit == 4) {
                 Piece p[2];
-                p[0].read_row(from);
-                p[1].read_row(from + 8 * kChunkPitch);
+                p[0].read(from, i, 0);
+                p[1].read(from, i, 8 * 128);
                 uint4 u[2];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
@@ -271,11 +258,12 @@ __device__ __forceinline__ void few_tokens_walk(uint8_t *smem, int cols, int til
                     mma_8<false>(c[1], lo[0], lo[1], hi[0], hi[1], q % 2 ? u[1].z : u[1].x, q % 2 ? u[1].w : u[1].y);
                 }
             } else { // a window of one or two octets
+                const uint32_t w = (from + (i >> 1) * kBoxBytes) ^ (i & 1) * 64;
 #pragma unroll 1
                 for (int q = q0; q < q0 + unit; ++q) {
                     const uint32_t x = (filled + (q - q0) / kRun == my_place ? x_here : zeros) + q * 8;
                     const uint2 u[2] = {read8u(x), read8u(x + term1)};
-                    const uint32_t wa = read4u(from + q * 4), wb = read4u(from + 8 * kChunkPitch + q * 4);
+                    const uint32_t wa = read4u(w + q * 4), wb = read4u(w + q * 4 + 8 * 128);
                     mma_8<true>(c[0], wa & 0x0f0f0f0fu, wb & 0x0f0f0f0fu, wa >> 4 & 0x0f0f0f0fu, wb >> 4 & 0x0f0f0f0fu, u[0].x, u[0].y);
                     mma_8<false>(c[1], wa & 0x0f0f0f0fu, wb & 0x0f0f0f0fu, wa >> 4 & 0x0f0f0f0fu, wb >> 4 & 0x0f0f0f0fu, u[1].x, u[1].y);
                 }
@@ -283,12 +271,8 @@ __device__ __forceinline__ void few_tokens_walk(uint8_t *smem, int cols, int til
             filled += unit / kRun;
         } else {
             Piece p[2];
-            p[0].read_row(from);
-            p[1].read_row(from + 8 * kChunkPitch);
-            if (kb == blocks - 1 && K % kKB != 0) {
-                p[0].cut(t, K - (blocks - 1) * kKB);
-                p[1].cut(t, K - (blocks - 1) * kKB);
-            }
+            p[0].read(from, i, 0);
+            p[1].read(from, i, 8 * 128);
             const uint32_t x = (FMT == kW16 ? g < cols : filled == my_place) ? x_here : zeros;
             Piece lo[2];
             if constexpr (kSplit) { // fp16 weights become the sum of two bf16, exactly
@@ -327,13 +311,12 @@ __device__ __forceinline__ void few_tokens_walk(uint8_t *smem, int cols, int til
         if (q0 == 4) { // the block is done
             q0 = 0;
             at += X::block_bytes(kTerms, cols);
-            from += kChunkRow / CB;
             --left;
             ++kb;
             if (++i == n) { // and the chunk
                 __syncwarp();
                 fetch_chunk(slot);
-                if (++slot == kTokenStages) {
+                if (++slot == kWeightSlots) {
                     slot = 0;
                     parity ^= 1;
                 }
@@ -376,7 +359,7 @@ __device__ __forceinline__ void few_tokens_walk(uint8_t *smem, int cols, int til
     }
     if (!ok) { // what is on its way lands before the CTA gives its memory back
         if (lane == 0) atomicExch(&g_few_status, 5);
-        for (int i = 0; i < kTokenStages; ++i) bar_wait(bars + i * 8, i < slot ? parity ^ 1 : parity);
+        for (int i = 0; i < kWeightSlots; ++i) bar_wait(bars + i * 8, i < slot ? parity ^ 1 : parity);
     }
     // columns of one token: their sums meet, then the shares'
 #pragma unroll
@@ -392,7 +375,7 @@ __device__ __forceinline__ void few_tokens_walk(uint8_t *smem, int cols, int til
     for (int j = 0; j < 2; ++j)
         if (2 * t + j < min(cols, tokens))
 #pragma unroll
-            for (int h = 0; h < 2; ++h) part[(warp * cols + 2 * t + j) * 17 + g + 8 * h] = acc[2 * h + j];
+            for (int h = 0; h < 2; ++h) part[(warp * cols + 2 * t + j) * 17 + lane_row() + 8 * h] = acc[2 * h + j];
     __syncthreads();
     if (share == 0 && tile < tiles)
         finish(tile, [&](int column, int row) {

@@ -211,52 +211,42 @@ __global__ void __launch_bounds__(256) int4_dequant_kernel(const uint4 *codes, c
 
 // ---- product of a few rows ----------------------------------------------------------------------------------------------
 struct Int4GemmArgs {
+    CUtensorMap map; // of the codes
     const void *x;
     int64_t ldx;
     ScaledRows xs;
     int M, N, K;
-    const uint8_t *codes;
     const __nv_bfloat16 *scale;
     const uint8_t *zero;
     const void *bias;
     void *out;
 };
 
-template <int G> struct Int4Rows { // a lane's two rows of the weight
-    const uint8_t *row[2];
-    RowScale<kWInt4> scale[2];
+template <int G> struct Int4Rows : LaneRows<kWInt4> { // the lane's rows of a tile of 16
     __device__ __forceinline__ void aim(const Int4GemmArgs &a, int n0) {
-        const int blocks = (a.K + kKB - 1) / kKB, groups = (a.K + G - 1) / G;
+        const int groups = (a.K + G - 1) / G;
+        row  = n0;
+        slab = 0;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int64_t r = min(n0 + (((int) threadIdx.x & 31) >> 2) + 8 * h, a.N - 1);
-            row[h]   = a.codes + r * blocks * kInt4BlockBytes;
+            const int64_t r = min(n0 + lane_row() + 8 * h, a.N - 1);
             scale[h] = {nullptr, (const uint16_t *) a.scale + r * groups, a.zero ? a.zero + r * groups : nullptr, 0, groups};
         }
     }
 };
 
 // Up to eight rows, as far as they fit into shared memory.
-template <int G> struct Int4TokenRows {
+template <int G> struct Int4TokenRows : Int4Rows<G> {
     const Int4GemmArgs &a;
-    const uint8_t *row;
-    RowScale<kWInt4> scale[2];
     __device__ __forceinline__ Int4TokenRows(const Int4GemmArgs &a) : a(a) {}
-    __device__ __forceinline__ void open(int tile, int) {
-        const int lane = threadIdx.x & 31, blocks = (a.K + kKB - 1) / kKB, groups = (a.K + G - 1) / G;
-        row = a.codes + (int64_t) min(tile * 16 + (lane & 15), a.N - 1) * blocks * kInt4BlockBytes;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int64_t r = min(tile * 16 + (lane >> 2) + 8 * h, a.N - 1);
-            scale[h] = {nullptr, (const uint16_t *) a.scale + r * groups, a.zero ? a.zero + r * groups : nullptr, 0, groups};
-        }
-    }
+    __device__ __forceinline__ void open(int tile, int) { this->aim(a, tile * 16); }
 };
 template <typename T, int G> __global__ void __launch_bounds__(32 * kTokenWarps, 1) int4_token_kernel(const __grid_constant__ Int4GemmArgs a, int shares) {
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ __align__(16) uint8_t raw[];
+    uint8_t *smem = aligned(raw);
     const int lane = threadIdx.x & 31, blocks = (a.K + kKB - 1) / kKB;
     few_tokens_walk<T, kWInt4, G, 2, false, false, false>(
-        smem, a.M, (a.N + 15) / 16, shares, 1, a.K, Int4TokenRows<G>(a),
+        smem, &a.map, a.M, (a.N + 15) / 16, shares, 1, a.K, Int4TokenRows<G>(a),
         [&](uint8_t *x, uint8_t *runs) {
             stage_blocks<T, T, kWInt4, G, 2>(x, runs, blocks, a.M, [&](int block, int col, int &left) {
                 left = a.K - block * kKB;
@@ -274,39 +264,65 @@ template <typename T, int G> __global__ void __launch_bounds__(32 * kTokenWarps,
         });
 }
 
-// More rows: a CTA has WR * 16 weight rows and up to NT * 8 rows of x; WK shares of k are added up in shared memory in a fixed order.
+// More rows: a CTA has WR * 16 weight rows and up to NT * 8 rows of x.  The CTAs of a cluster share k; each adds up, and writes, its part of the
+// results, in the order of k.
 template <int G> struct Int4BatchRows : Int4Rows<G> {
     ScaledRows xs;
     int row0;
     __device__ __forceinline__ const uint8_t *x(int, int col) const { return xs.planes + (row0 + col) * xs.pitch; }
-    __device__ __forceinline__ const float *runs(int col) const { return xs.runs + (int64_t) (row0 + col) * xs.blocks; }
 };
-template <typename T, int G, int NT, int WR, int WK, int kStages>
-__global__ void __launch_bounds__(32 * WR * WK, 2) int4_gemm_kernel(const Int4GemmArgs a) {
-    extern __shared__ __align__(16) uint8_t smem[];
-    using W = Walk<kWInt4, 128, WR, WK>;
-    const int n0 = blockIdx.x * W::kRows, m0 = blockIdx.y * (NT * 8), cols = min(NT * 8, a.M - m0);
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float read_peer(const float *p, uint32_t rank) {
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(shared_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+template <typename T, int G, int NT, int WR>
+__global__ void __launch_bounds__(32 * WR, 16 / WR) int4_gemm_kernel(const __grid_constant__ Int4GemmArgs a, int shares) {
+    extern __shared__ __align__(16) uint8_t raw[];
+    uint8_t *smem = aligned(raw);
+    using W = Walk<kWInt4, NT, WR>;
+    __shared__ uint64_t bars[W::kBars];
+    const int tile = blockIdx.x / shares, share = blockIdx.x % shares; // (the rank in the cluster)
+    const int n0 = tile * W::kRows, m0 = blockIdx.y * (NT * 8), cols = min(NT * 8, a.M - m0);
+    const int blocks = (a.K + kKB - 1) / kKB, chunks = (blocks + kChunk<kWInt4> - 1) / kChunk<kWInt4>;
     Int4BatchRows<G> src;
-    src.aim(a, n0 + (threadIdx.x >> 5) % WR * 16);
+    src.aim(a, n0 + (threadIdx.x >> 5) * 16);
     src.xs   = a.xs;
     src.row0 = m0;
     float acc[NT][4] = {};
-    few_rows_walk<T, kWInt4, G, 128, NT, WR, WK, kStages, 1, false>(acc, smem, a.K, cols, (cols + 7) / 8, src);
-    const ShareSums<NT, WR, WK> sums(acc, smem);
-    for (int i = threadIdx.x; i < cols * W::kRows; i += W::kThreads) {
+    few_rows_walk<T, kWInt4, G, 128, NT, WR, 1, false>(acc, smem, bars, &a.map, a.K, cols, share * chunks / shares * kChunk<kWInt4>,
+                                                       min(blocks, (share + 1) * chunks / shares * kChunk<kWInt4>), src);
+    const RowSums<kWInt4, NT, WR> sums(acc, smem);
+    if (shares > 1) cluster_sync();
+    for (int i = threadIdx.x + share * W::kThreads; i < cols * W::kRows; i += W::kThreads * shares) {
         const int m = i / W::kRows, n = i % W::kRows;
         if (n0 + n >= a.N) continue;
-        float s = sums.sum(m, n);
+        float s = 0.0f;
+        if (shares == 1) s = sums.sum(m, n);
+        else for (int r = 0; r < shares; ++r) s += read_peer(&sums.part[m * sums.kPitch + n], r);
         if (a.bias != nullptr) s += to_f32(((const T *) a.bias)[n0 + n]);
         ((T *) a.out)[(int64_t) (m0 + m) * a.N + n0 + n] = from_f32<T>(s);
     }
+    if (shares > 1) cluster_sync(); // nobody leaves while his sums are read
 }
 
-template <typename T, int G, int NT, int WR, int WK, int kStages> cudaError_t launch_tile(const Int4GemmArgs &a, cudaStream_t st) {
-    using W = Walk<kWInt4, 128, WR, WK>;
-    const int smem = W::template smem<NT>(kStages, 1, (int) imin(a.M, NT * 8));
-    return launch_early(int4_gemm_kernel<T, G, NT, WR, WK, kStages>, dim3((unsigned) cdiv(a.N, W::kRows), (unsigned) cdiv(a.M, NT * 8)), W::kThreads,
-                        (size_t) smem, st, a);
+template <typename T, int G, int NT, int WR> int launch_tile(const Int4GemmArgs &a, cudaStream_t st) {
+    using W = Walk<kWInt4, NT, WR>;
+    int sms = 0;
+    if (int rc = sm_count(&sms)) return rc;
+    const int tiles = cdiv(a.N, W::kRows), sets = cdiv(a.M, NT * 8), chunks = cdiv(a.K, kKB * kChunk<kWInt4>);
+    int shares = 1; // of k: as many as it takes to give every SM its 16 warps
+    while (shares < 8 && 2 * shares <= chunks && (int64_t) tiles * sets * shares * 2 <= (int64_t) sms * (16 / WR)) shares *= 2;
+    PTB_CUDA(launch_early(int4_gemm_kernel<T, G, NT, WR>, dim3((unsigned) (tiles * shares), (unsigned) sets), W::kThreads,
+                          (size_t) W::smem(1, (int) imin(a.M, NT * 8)), st, (unsigned) shares, a, shares));
+    PTB_LAUNCH_CHECK("int4_gemm_kernel");
+    return 0;
 }
 
 constexpr int kMostSmem = 227 * 1024 - 1024; // of a CTA, less what is not dynamic
@@ -317,18 +333,16 @@ template <typename T, int G> int launch_gemm(const Int4GemmArgs &a, cudaStream_t
         int sms = 0;
         if (int rc = sm_count(&sms)) return rc;
         const int tiles = cdiv(a.N, 16), shares = token_shares(tiles, cdiv(a.K, kKB), sms);
-        PTB_CUDA(launch_early(int4_token_kernel<T, G>, dim3((unsigned) cdiv(tiles, kTokenWarps >> shares)), 32 * kTokenWarps, (size_t) token_smem(x_bytes, a.M), st, a, shares));
+        PTB_CUDA(launch_early(int4_token_kernel<T, G>, dim3((unsigned) cdiv(tiles, kTokenWarps >> shares)), 32 * kTokenWarps, (size_t) token_smem(x_bytes, a.M), st, 1, a, shares));
         PTB_LAUNCH_CHECK("int4_token_kernel");
         return 0;
     }
     const int64_t warps = a.M * cdiv<int64_t>(a.K, kKB);
-    PTB_CUDA(launch_early(scale_rows_kernel<T, kWInt4>, dim3((unsigned) cdiv<int64_t>(warps, 4)), 128, 0, st, (const T *) a.x, a.ldx, a.M, a.K, a.xs));
+    PTB_CUDA(launch_early(scale_rows_kernel<T, kWInt4>, dim3((unsigned) cdiv<int64_t>(warps, 4)), 128, 0, st, 1, (const T *) a.x, a.ldx, a.M, a.K, a.xs));
     PTB_LAUNCH_CHECK("scale_rows_kernel");
-    if (a.M <= 8) PTB_CUDA((launch_tile<T, G, 1, 2, 4, 4>(a, st)));
-    else if (a.M <= 16) PTB_CUDA((launch_tile<T, G, 2, 4, 2, 4>(a, st)));
-    else PTB_CUDA((launch_tile<T, G, 4, 4, 2, 4>(a, st)));
-    PTB_LAUNCH_CHECK("int4_gemm_kernel");
-    return 0;
+    if (a.M <= 8) return launch_tile<T, G, 1, 4>(a, st);
+    if (a.M <= 16) return launch_tile<T, G, 2, 4>(a, st);
+    return a.M <= 32 ? launch_tile<T, G, 4, 8>(a, st) : launch_tile<T, G, 8, 16>(a, st);
 }
 
 bool is_group(int64_t g) { return g == 32 || g == 64 || g == 128; }
@@ -396,7 +410,7 @@ int ptb_dequant_int4(const void *codes, const void *scale, const void *zero, int
 
 int64_t ptb_gemm_int4_workspace(int dtype, int64_t M, int64_t K, int64_t group) {
     if (M < 0 || K < 1 || (dtype != PTB_BF16 && dtype != PTB_F16) || !is_group(group)) return -1;
-    return scaled_bytes(1, M, K, 128);
+    return scaled_bytes(1, M, K);
 }
 
 int ptb_gemm_int4(const void *x, int dtype, int64_t ldx, int64_t M, int64_t N, int64_t K, const void *codes, const void *scale, const void *zero,
@@ -410,8 +424,8 @@ int ptb_gemm_int4(const void *x, int dtype, int64_t ldx, int64_t M, int64_t N, i
     if (M == 0 || N == 0) return 0;
     PTB_REQUIRE(x && codes && scale && workspace && out, PTB_ERR_ARG, "gemm_int4: null pointer");
     PTB_REQUIRE(aligned16(x) && aligned16(codes) && aligned16(workspace), PTB_ERR_ALIGN, "gemm_int4: x, the codes and the workspace must be 16-byte aligned");
-    const Int4GemmArgs a{x, ldx, scaled_rows_at(workspace, 1, M, K), (int) M, (int) N, (int) K, (const uint8_t *) codes,
-                         (const __nv_bfloat16 *) scale, (const uint8_t *) zero, bias, out};
+    Int4GemmArgs a{{}, x, ldx, scaled_rows_at(workspace, M, K), (int) M, (int) N, (int) K, (const __nv_bfloat16 *) scale, (const uint8_t *) zero, bias, out};
+    if (int rc = weight_map(&a.map, codes, cdiv<int64_t>(K, kKB) * kInt4BlockBytes, N, 1, false)) return rc;
     cudaStream_t st = (cudaStream_t) stream;
     PTB_SWITCH_INT4_GROUP(group, G, return dtype == PTB_BF16 ? launch_gemm<__nv_bfloat16, G>(a, st) : launch_gemm<__half, G>(a, st));
     return 0;

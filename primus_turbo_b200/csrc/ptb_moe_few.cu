@@ -27,8 +27,7 @@ constexpr int kMaxExperts = 1024;
 
 // One expert-major weight [E, rows, K].
 struct ExpertWeight {
-    const uint8_t *data;
-    int64_t row_bytes, expert_bytes;
+    CUtensorMap map;
     const void *scale; // fp32 (8-bit) or bf16 (4-bit)
     const uint8_t *zero;
     int64_t scale_expert; // elements from expert to expert
@@ -210,38 +209,37 @@ __device__ __forceinline__ void find_pairs(const LayerArgs &a, Pairs &out) {
     }
 }
 
-template <int FMT> struct ExpertRows { // a lane's two rows of an expert's weight
-    const uint8_t *row[2];
-    RowScale<FMT> scale[2];
-    __device__ __forceinline__ void aim(const ExpertWeight &w, int64_t e, int r0, int r1, int rows) {
-        row[0]   = w.data + e * w.expert_bytes + r0 * w.row_bytes;
-        row[1]   = w.data + e * w.expert_bytes + r1 * w.row_bytes;
-        scale[0] = row_scale<FMT>(w, e, r0, rows);
-        scale[1] = row_scale<FMT>(w, e, r1, rows);
-    }
-};
+// The warp's rows of expert e: eight gate rows from r0 on and the up rows that go with them, or 16 rows of the down weight.
+template <int FMT> __device__ __forceinline__ void aim_gate_up(LaneRows<FMT> &out, const ExpertWeight &w, int64_t e, int r0, int I) {
+    const int r  = min(r0 + lane_row(), I - 1);
+    out.row      = r0;
+    out.slab     = (int) e * 2;
+    out.scale[0] = row_scale<FMT>(w, e, r, 2 * I);
+    out.scale[1] = row_scale<FMT>(w, e, I + r, 2 * I);
+}
+template <int FMT> __device__ __forceinline__ void aim_down(LaneRows<FMT> &out, const ExpertWeight &w, int64_t e, int r0, int H) {
+    const int r  = r0 + lane_row();
+    out.row      = r0;
+    out.slab     = (int) e;
+    out.scale[0] = row_scale<FMT>(w, e, min(r, H - 1), H);
+    out.scale[1] = row_scale<FMT>(w, e, min(r + 8, H - 1), H);
+}
 
-template <int FMT> struct TokenRows { // row lane % 16 of a tile, and the scales of rows lane / 4 and lane / 4 + 8
-    const uint8_t *row;
-    RowScale<FMT> scale[2];
-};
-template <int FMT> struct GateUpTokenRows : TokenRows<FMT> {
+template <int FMT> struct GateUpTokenRows : LaneRows<FMT> {
     const LayerArgs &a;
     const Pairs &pairs;
     int tiles; // of an expert
     __device__ __forceinline__ GateUpTokenRows(const LayerArgs &a, const Pairs &pairs, int tiles) : a(a), pairs(pairs), tiles(tiles) {}
     __device__ __forceinline__ void open(int tile, int) {
-        const int hit = tile / tiles, r0 = (tile - hit * tiles) * 8, lane = threadIdx.x & 31, r = min(r0 + (lane >> 2), a.I - 1);
-        const int64_t e = pairs.expert[hit];
-        this->row = a.w1.data + e * a.w1.expert_bytes + (min(r0 + (lane & 7), a.I - 1) + (lane & 8 ? a.I : 0)) * a.w1.row_bytes;
-        this->scale[0] = row_scale<FMT>(a.w1, e, r, 2 * a.I);
-        this->scale[1] = row_scale<FMT>(a.w1, e, a.I + r, 2 * a.I);
+        const int hit = tile / tiles;
+        aim_gate_up<FMT>(*this, a.w1, pairs.expert[hit], (tile - hit * tiles) * 8, a.I);
     }
 };
 
 template <typename T, int FMT, int G>
 __global__ void __launch_bounds__(32 * kTokenWarps, 1) moe_gate_up_token_kernel(const __grid_constant__ LayerArgs a, int shares) {
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ __align__(16) uint8_t raw[];
+    uint8_t *smem = aligned(raw);
     __shared__ Pairs pairs;
     grid_dep_wait(); // the kernel before this one is somebody else's
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tiles = (a.I + 7) / 8, blocks = (a.H + kKB - 1) / kKB;
@@ -249,7 +247,7 @@ __global__ void __launch_bounds__(32 * kTokenWarps, 1) moe_gate_up_token_kernel(
     if (warp == 0) find_pairs(a, pairs);
     __syncthreads();
     few_tokens_walk<T, FMT, G, kTerms, false, false, false>(
-        smem, a.T, pairs.hits * tiles, shares, 1, a.H, GateUpTokenRows<FMT>(a, pairs, tiles),
+        smem, &a.w1.map, a.T, pairs.hits * tiles, shares, 1, a.H, GateUpTokenRows<FMT>(a, pairs, tiles),
         [&](uint8_t *x, uint8_t *runs) {
             stage_blocks<T, T, FMT, G, kTerms>(x, runs, blocks, a.T, [&](int block, int col, int &left) {
                 left = a.H - block * kKB;
@@ -265,16 +263,12 @@ __global__ void __launch_bounds__(32 * kTokenWarps, 1) moe_gate_up_token_kernel(
         });
 }
 
-template <int FMT> struct DownTokenRows : TokenRows<FMT> {
+template <int FMT> struct DownTokenRows : LaneRows<FMT> {
     const LayerArgs &a;
     const Pairs &pairs;
     __device__ __forceinline__ DownTokenRows(const LayerArgs &a, const Pairs &pairs) : a(a), pairs(pairs) {}
     __device__ __forceinline__ void open(int tile, int segment) {
-        const int lane = threadIdx.x & 31, r = tile * 16 + (lane >> 2);
-        const int64_t e = pairs.expert[segment];
-        this->row = a.w2.data + e * a.w2.expert_bytes + min(tile * 16 + (lane & 15), a.H - 1) * a.w2.row_bytes;
-        this->scale[0] = row_scale<FMT>(a.w2, e, min(r, a.H - 1), a.H);
-        this->scale[1] = row_scale<FMT>(a.w2, e, min(r + 8, a.H - 1), a.H);
+        aim_down<FMT>(*this, a.w2, pairs.expert[segment], tile * 16, a.H);
     }
     __device__ __forceinline__ bool mask(int segment, int column) const { return pairs.slot[segment * kTokenCols + column] >= 0; }
 };
@@ -284,7 +278,8 @@ template <typename T, int FMT> constexpr int kHTerms = FMT == kW16 || FMT == kWI
 
 template <typename T, int FMT, int G>
 __global__ void __launch_bounds__(32 * kTokenWarps, 1) moe_down_token_kernel(const __grid_constant__ LayerArgs a, int shares) {
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ __align__(16) uint8_t raw[];
+    uint8_t *smem = aligned(raw);
     __shared__ Pairs pairs;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, blocks = (a.I + kKB - 1) / kKB;
     // 16-bit weights: the MMA's type is that of h, bf16, whatever x is
@@ -293,7 +288,7 @@ __global__ void __launch_bounds__(32 * kTokenWarps, 1) moe_down_token_kernel(con
     if (warp == 0) find_pairs(a, pairs);
     __syncthreads();
     few_tokens_walk<M, FMT, G, kTerms, FMT == kW16 && std::is_same<T, __half>::value, true, true>(
-        smem, a.T, (a.H + 15) / 16, shares, pairs.hits, a.I, DownTokenRows<FMT>(a, pairs),
+        smem, &a.w2.map, a.T, (a.H + 15) / 16, shares, pairs.hits, a.I, DownTokenRows<FMT>(a, pairs),
         [&](uint8_t *x, uint8_t *runs) {
             stage_blocks<M, float, FMT, G, kTerms>(x, runs, pairs.hits * blocks, a.T, [&](int block, int col, int &left) {
                 const int hit = block / blocks, kb = block - hit * blocks, slot = pairs.slot[hit * kTokenCols + col];
@@ -310,48 +305,45 @@ __global__ void __launch_bounds__(32 * kTokenWarps, 1) moe_down_token_kernel(con
 }
 
 // ---- more tokens: gate and up projection -----------------------------------------------------------------------------------------
-constexpr int kChannels = 64; // of a CTA: eight warps of eight
+constexpr int kWarps = 8, kChannels = 8 * kWarps; // of a CTA, eight channels a warp
 
-template <int FMT> struct GateUpRows : ExpertRows<FMT> {
+template <int FMT> struct GateUpRows : LaneRows<FMT> {
     const uint8_t *x0;
     int64_t pitch;
-    const float *runs0;
-    int blocks;
     const int *token; // row of x of a column
     __device__ __forceinline__ const uint8_t *x(int, int col) const { return x0 + token[col] * pitch; }
-    __device__ __forceinline__ const float *runs(int col) const { return runs0 + (int64_t) token[col] * blocks; }
 };
 
 // blockIdx.y counts the experts that are hit.
-template <typename T, int FMT, int G, int NT, int kStages>
-__global__ void __launch_bounds__(256, 2) moe_gate_up_kernel(const LayerArgs a) {
-    extern __shared__ __align__(16) uint8_t smem[];
-    using W = Walk<FMT, 128, 8, 1>;
+template <typename T, int FMT, int G, int NT>
+__global__ void __launch_bounds__(32 * kWarps, 2) moe_gate_up_kernel(const __grid_constant__ LayerArgs a) {
+    extern __shared__ __align__(16) uint8_t raw[];
+    uint8_t *smem = aligned(raw);
+    using W = Walk<FMT, NT, kWarps>;
     constexpr int kPitch = kChannels + 1;
+    __shared__ uint64_t bars[W::kBars];
     __shared__ int token[NT * 8];
-    __shared__ float h_of[kScaledX<FMT> ? NT * 8 * kPitch : 1];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
+    float *h_of = reinterpret_cast<float *>(smem + W::kSums); // [column][channel]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     grid_dep_wait();
     const int hit = blockIdx.y;
     if (hit >= a.lists.active[0]) return;
     const int64_t e = a.lists.active[1 + hit];
     const int begin = a.lists.first[hit], end = a.lists.first[hit + 1];
-    const int r0 = blockIdx.x * kChannels, row = min(r0 + warp * 8 + g, a.I - 1);
+    const int r0 = blockIdx.x * kChannels;
     GateUpRows<FMT> src;
-    src.aim(a.w1, e, row, a.I + row, 2 * a.I);
-    src.x0     = kScaledX<FMT> ? a.xs.planes : (const uint8_t *) a.x;
-    src.pitch  = kScaledX<FMT> ? a.xs.pitch : a.ldx * 2;
-    src.runs0  = a.xs.runs;
-    src.blocks = a.xs.blocks;
-    src.token  = token;
+    aim_gate_up<FMT>(src, a.w1, e, r0 + warp * 8, a.I);
+    src.x0    = kScaledX<FMT> ? a.xs.planes : (const uint8_t *) a.x;
+    src.pitch = kScaledX<FMT> ? a.xs.pitch : a.ldx * 2;
+    src.token = token;
     for (int s0 = begin; s0 < end; s0 += NT * 8) {
         const int cols = min(NT * 8, end - s0);
         if (threadIdx.x < cols) token[threadIdx.x] = a.lists.token[s0 + threadIdx.x];
         __syncthreads();
         float acc[NT][4] = {};
-        if (r0 < a.I) few_rows_walk<T, FMT, G, 128, NT, 8, 1, kStages, 1, false>(acc, smem, a.H, cols, (cols + 7) / 8, src);
+        if (r0 < a.I) few_rows_walk<T, FMT, G, 128, NT, kWarps, 1, false>(acc, smem, bars, &a.w1.map, a.H, cols, 0, (a.H + kKB - 1) / kKB, src);
         else grid_dep_open(); // (past the last channel there is only h's padding to write)
-        const ShareSums<NT, 8, 1> sums(acc, smem);
+        const RowSums<FMT, NT, kWarps> sums(acc, smem);
         for (int i = threadIdx.x; i < cols * kChannels; i += W::kThreads) {
             const int c = i / kChannels, r = i % kChannels, at = r / 8 * 16 + r % 8, slot = s0 + c;
             const float h = r0 + r < a.I ? swiglu_prob(sums.sum(c, at), sums.sum(c, at + 8), a.lists.prob[slot]) : 0.0f;
@@ -365,7 +357,7 @@ __global__ void __launch_bounds__(256, 2) moe_gate_up_kernel(const LayerArgs a) 
         }
         if constexpr (kScaledX<FMT>) { // a half-warp scales a token's 64 channels, four a lane
             __syncthreads();
-            for (int c2 = warp; 2 * c2 < cols; c2 += 8) {
+            for (int c2 = warp; 2 * c2 < cols; c2 += kWarps) {
                 const int c = min(2 * c2 + (lane >> 4), cols - 1), in = (lane & 15) * 4;
                 const int64_t slot = s0 + c;
                 float v[4], largest = 0.0f, scale, inv;
@@ -377,20 +369,10 @@ __global__ void __launch_bounds__(256, 2) moe_gate_up_kernel(const LayerArgs a) 
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
                 block_scale(largest, kTopHalf, scale, inv);
-                uint8_t *to = a.hs.planes + slot * a.hs.pitch + (r0 + in) * 2;
+                uint8_t *block = a.hs.planes + slot * a.hs.pitch + (int64_t) (r0 / kKB) * kScaledBlock;
 #pragma unroll
-                for (int term = 0; term < kHScaled<T>; ++term) {
-                    __half h[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float s = v[j] * inv;
-                        h[half_place<FMT>(j)] = term == 0 ? __float2half_rn(s) : __float2half_rn(fabsf(s) < INFINITY ? s - __half2float(__float2half_rn(s)) : 0.0f);
-                    }
-                    uint2 u;
-                    memcpy(&u, h, 8);
-                    *reinterpret_cast<uint2 *>(to + term * a.hs.plane) = u;
-                }
-                if ((lane & 15) == 0) a.hs.runs[slot * a.hs.blocks * 2 + r0 / 64] = scale;
+                for (int term = 0; term < kHScaled<T>; ++term) put_halves<FMT>(block + term * a.hs.plane, r0 % kKB + in, v, inv, term > 0);
+                if ((lane & 15) == 0) reinterpret_cast<float *>(block + 256)[r0 % kKB / 64] = scale;
             }
         }
         if (s0 + NT * 8 < end) __syncthreads(); // all of this is read before it is written again
@@ -398,41 +380,40 @@ __global__ void __launch_bounds__(256, 2) moe_gate_up_kernel(const LayerArgs a) 
 }
 
 // ---- more tokens: down projection, a row per pair --------------------------------------------------------------------------------
-template <int FMT> struct DownRows : ExpertRows<FMT> {
+template <int FMT> struct DownRows : LaneRows<FMT> {
     const uint8_t *x0;
     int64_t plane, pitch;
-    const float *runs0;
-    int blocks;
     __device__ __forceinline__ const uint8_t *x(int term, int col) const { return x0 + term * plane + col * pitch; }
-    __device__ __forceinline__ const float *runs(int col) const { return runs0 + (int64_t) col * blocks * 2; }
 };
 
-template <typename T, int FMT, int G, int NT, int kStages>
-__global__ void __launch_bounds__(256, 2) moe_down_kernel(const LayerArgs a) {
-    extern __shared__ __align__(16) uint8_t smem[];
-    using W = Walk<FMT, 64, 8, 1>;
+template <typename T, int FMT> constexpr int kDownTerms = kScaledX<FMT> ? kHScaled<T> : 2;
+// Two terms of 32 columns leave shared memory for one CTA an SM: that one has 16 warps.
+template <typename T, int FMT, int NT> constexpr int kDownWarps = NT > 2 && kDownTerms<T, FMT> == 2 ? 16 : 8;
+
+template <typename T, int FMT, int G, int NT, int WR>
+__global__ void __launch_bounds__(32 * WR, 16 / WR) moe_down_kernel(const __grid_constant__ LayerArgs a) {
+    extern __shared__ __align__(16) uint8_t raw[];
+    uint8_t *smem = aligned(raw);
+    using W = Walk<FMT, NT, WR>;
+    __shared__ uint64_t bars[W::kBars];
     const int hit = blockIdx.y; // the lists are from two kernels before
     if (hit >= a.lists.active[0]) {
         grid_dep_wait();
         return;
     }
-    const int warp = threadIdx.x >> 5, g = (threadIdx.x & 31) >> 2;
-    const int64_t e = a.lists.active[1 + hit];
+    const int warp = threadIdx.x >> 5, n0 = blockIdx.x * W::kRows;
     const int begin = a.lists.first[hit], end = a.lists.first[hit + 1];
-    const int n0 = blockIdx.x * W::kRows, row = n0 + warp * 16 + g;
     DownRows<FMT> src;
-    src.aim(a.w2, e, min(row, a.H - 1), min(row + 8, a.H - 1), a.H);
-    src.plane  = kScaledX<FMT> ? a.hs.plane : (int64_t) ((const uint8_t *) a.h_lo - (const uint8_t *) a.h_hi);
-    src.pitch  = kScaledX<FMT> ? a.hs.pitch : (int64_t) a.I * 2;
-    src.blocks = a.hs.blocks;
+    aim_down<FMT>(src, a.w2, a.lists.active[1 + hit], n0 + warp * 16, a.H);
+    src.plane = kScaledX<FMT> ? a.hs.plane : (int64_t) ((const uint8_t *) a.h_lo - (const uint8_t *) a.h_hi);
+    src.pitch = kScaledX<FMT> ? a.hs.pitch : (int64_t) a.I * 2;
     for (int s0 = begin; s0 < end; s0 += NT * 8) {
         const int cols = min(NT * 8, end - s0);
-        src.x0    = (kScaledX<FMT> ? a.hs.planes : (const uint8_t *) a.h_hi) + s0 * src.pitch;
-        src.runs0 = a.hs.runs + (int64_t) s0 * src.blocks * 2;
+        src.x0 = (kScaledX<FMT> ? a.hs.planes : (const uint8_t *) a.h_hi) + s0 * src.pitch;
         float acc[NT][4] = {};
-        few_rows_walk<__nv_bfloat16, FMT, G, 64, NT, 8, 1, kStages, kScaledX<FMT> ? kHScaled<T> : 2, FMT == kW16 && std::is_same<T, __half>::value>(
-            acc, smem, a.I, cols, (cols + 7) / 8, src);
-        const ShareSums<NT, 8, 1> sums(acc, smem);
+        few_rows_walk<__nv_bfloat16, FMT, G, 64, NT, WR, kDownTerms<T, FMT>, FMT == kW16 && std::is_same<T, __half>::value>(
+            acc, smem, bars, &a.w2.map, a.I, cols, 0, (a.I + kKB - 1) / kKB, src);
+        const RowSums<FMT, NT, WR> sums(acc, smem);
         for (int i = threadIdx.x; i < cols * W::kRows; i += W::kThreads) {
             const int c = i / W::kRows, n = i % W::kRows;
             if (n0 + n < a.H) a.rows[(int64_t) (s0 + c) * a.H + n0 + n] = sums.sum(c, n);
@@ -462,8 +443,6 @@ template <typename T> __global__ void __launch_bounds__(128) moe_merge_kernel(co
     for (int j = 0; j < 8; ++j) ((T *) a.out)[(int64_t) token * a.H + n + j] = from_f32<T>(s[j]);
 }
 
-#define PTB_EARLY(name, kernel, ...)                         do {                                                         PTB_CUDA(launch_early(kernel, __VA_ARGS__));             PTB_LAUNCH_CHECK(name);                              } while (0)
-
 constexpr int kMostSmem = 227 * 1024 - 4096; // of a CTA, less what is not dynamic
 
 // Whether the two-kernel form has room for x and for h, and the shared memory of its kernels.
@@ -480,34 +459,38 @@ template <typename T, int FMT, int G> int launch_token(const LayerArgs &a, int u
     const int hits = (int) imin(a.E, a.T * a.k), up_tiles = hits * cdiv(a.I, 8), down_tiles = cdiv(a.H, 16);
     const int up_shares = token_shares(up_tiles, cdiv(a.H, kKB), sms), down_shares = token_shares(down_tiles, hits * cdiv(a.I, kKB), sms);
     const dim3 g1((unsigned) cdiv(up_tiles, kTokenWarps >> up_shares)), g2((unsigned) cdiv(down_tiles, kTokenWarps >> down_shares));
-    PTB_CUDA(launch_early(moe_gate_up_token_kernel<T, FMT, G>, g1, 32 * kTokenWarps, (size_t) up, st, a, up_shares));
+    PTB_CUDA(launch_early(moe_gate_up_token_kernel<T, FMT, G>, g1, 32 * kTokenWarps, (size_t) up, st, 1, a, up_shares));
     PTB_LAUNCH_CHECK("moe_gate_up_token_kernel");
-    PTB_CUDA(launch_early(moe_down_token_kernel<T, FMT, G>, g2, 32 * kTokenWarps, (size_t) down, st, a, down_shares));
+    PTB_CUDA(launch_early(moe_down_token_kernel<T, FMT, G>, g2, 32 * kTokenWarps, (size_t) down, st, 1, a, down_shares));
     PTB_LAUNCH_CHECK("moe_down_token_kernel");
     return 0;
 }
 
-
 template <typename T, int FMT, int G, int NT> int launch_batch(const LayerArgs &a, cudaStream_t st) {
-    constexpr int S = FMT == kWInt4 ? 5 : FMT == kW16 ? 2 : 4, D = FMT == kWInt4 ? 5 : FMT == kW16 ? 2 : 4;
+    constexpr int kDown = kDownWarps<T, FMT, NT>;
+    using W = Walk<FMT, NT, kWarps>;
+    using D = Walk<FMT, NT, kDown>;
     const unsigned hits = (unsigned) imin(a.E, a.T * a.k), splits = kScaledX<FMT> ? (unsigned) cdiv(a.T * cdiv(a.H, kKB), 32) : 0u;
     const int cols = (int) imin(a.T, NT * 8);
-    PTB_EARLY("moe_list_kernel", (moe_list_kernel<T, FMT>), dim3(1 + splits), 1024, 0, st, a.ids, a.probs, a.T, a.k, a.E, a.lists, (const T *) a.x, a.ldx, a.H, a.xs);
-    using U = Walk<FMT, 128, 8, 1>;
-    PTB_EARLY("moe_gate_up_kernel", (moe_gate_up_kernel<T, FMT, G, NT, S>),
-              dim3((unsigned) (kScaledX<FMT> ? cdiv(a.I, kKB) * 2 : cdiv(a.I, kChannels)), hits), U::kThreads, (U::template smem<NT>(S, 1, cols)), st, a); // h's planes are whole blocks
-    using W = Walk<FMT, 64, 8, 1>;
-    PTB_EARLY("moe_down_kernel", (moe_down_kernel<T, FMT, G, NT, D>), dim3((unsigned) cdiv(a.H, W::kRows), hits), W::kThreads,
-              (W::template smem<NT>(D, kScaledX<FMT> ? kHScaled<T> : 2, cols)), st, a);
-    PTB_EARLY("moe_merge_kernel", moe_merge_kernel<T>, dim3((unsigned) cdiv(a.H, 1024), (unsigned) a.T), 128, 0, st, a);
+    const int up_smem = W::smem(1, cols, NT * 8 * (kChannels + 1) * 4), down_smem = D::smem(kDownTerms<T, FMT>, cols);
+    PTB_CUDA(launch_early(moe_list_kernel<T, FMT>, dim3(1 + splits), 1024, 0, st, 1, a.ids, a.probs, a.T, a.k, a.E, a.lists, (const T *) a.x, a.ldx, a.H, a.xs));
+    PTB_LAUNCH_CHECK("moe_list_kernel");
+    const unsigned channels = (unsigned) (kScaledX<FMT> ? cdiv(a.I, kKB) * 2 : cdiv(a.I, kChannels)); // CTAs; h's planes are whole blocks
+    PTB_CUDA(launch_early(moe_gate_up_kernel<T, FMT, G, NT>, dim3(channels, hits), W::kThreads, (size_t) up_smem, st, 1, a));
+    PTB_LAUNCH_CHECK("moe_gate_up_kernel");
+    PTB_CUDA(launch_early(moe_down_kernel<T, FMT, G, NT, kDown>, dim3((unsigned) cdiv(a.H, D::kRows), hits), D::kThreads, (size_t) down_smem, st, 1, a));
+    PTB_LAUNCH_CHECK("moe_down_kernel");
+    PTB_CUDA(launch_early(moe_merge_kernel<T>, dim3((unsigned) cdiv(a.H, 1024), (unsigned) a.T), 128, 0, st, 1, a));
+    PTB_LAUNCH_CHECK("moe_merge_kernel");
     return 0;
 }
 
 template <typename T, int FMT, int G> int launch_layer(const LayerArgs &a, cudaStream_t st) {
     int up = 0, down = 0;
     if (fits_token<T, FMT, G>(a, up, down)) return launch_token<T, FMT, G>(a, up, down, st);
+    // columns of a CTA: an expert with more reads its weight again
     if (a.T <= 8) return launch_batch<T, FMT, G, 1>(a, st);
-    return a.T <= 16 ? launch_batch<T, FMT, G, 2>(a, st) : launch_batch<T, FMT, G, 4>(a, st);
+    return a.T <= 16 || a.T * a.k <= 10 * a.E ? launch_batch<T, FMT, G, 2>(a, st) : launch_batch<T, FMT, G, 4>(a, st);
 }
 
 template <typename T> int launch_format(int format, int group, const LayerArgs &a, cudaStream_t st) {
@@ -530,8 +513,8 @@ Pieces pieces(int format, int dtype, int64_t T, int64_t k, int64_t H, int64_t I)
     auto up = [](int64_t n) { return (n + 15) / 16 * 16; };
     const bool scaled = format == PTB_E4M3 || format == PTB_E5M2 || format == PTB_INT4;
     Pieces p{};
-    p.hs    = scaled ? up(scaled_bytes(1, T, H, 128)) : 0;
-    p.rows  = p.hs + up(imax(scaled ? scaled_bytes(dtype == PTB_F16 ? 2 : 1, T * k, I, 64) : 0, T * k * I * 4));
+    p.hs    = scaled ? up(scaled_bytes(1, T, H)) : 0;
+    p.rows  = p.hs + up(imax(scaled ? scaled_bytes(dtype == PTB_F16 ? 2 : 1, T * k, I) : 0, T * k * I * 4));
     p.lists = p.rows + up(T * k * H * 4);
     p.total = p.lists + list_words(T * k) * 4;
     return p;
@@ -541,10 +524,7 @@ Pieces pieces(int format, int dtype, int64_t T, int64_t k, int64_t H, int64_t I)
 int describe(const char *who, const PtbExpertWeight &p, int format, int64_t rows, int64_t K, ExpertWeight &w) {
     PTB_REQUIRE(p.data != nullptr, PTB_ERR_ARG, "moe_few_tokens: %s has no data", who);
     PTB_REQUIRE(aligned16(p.data), PTB_ERR_ALIGN, "moe_few_tokens: %s must be 16-byte aligned", who);
-    w      = ExpertWeight{};
-    w.data = (const uint8_t *) p.data;
-    w.row_bytes = format == PTB_INT4 ? cdiv<int64_t>(K, kKB) * kInt4BlockBytes : format == PTB_E4M3 || format == PTB_E5M2 ? K : 2 * K;
-    w.expert_bytes = w.row_bytes * rows;
+    w = ExpertWeight{};
     if (format == PTB_INT4) {
         PTB_REQUIRE(p.group == 32 || p.group == 64 || p.group == 128, PTB_ERR_ARG, "moe_few_tokens: %s: the group size must be 32, 64 or 128", who);
         w.groups = (int) cdiv<int64_t>(K, p.group);
@@ -603,12 +583,15 @@ int ptb_moe_few_tokens(const void *x, int dtype, int64_t ldx, int64_t T, int64_t
     LayerArgs a{};
     if (int rc = describe("the gate and up weight", *gate_up, format, 2 * I, H, a.w1)) return rc;
     if (int rc = describe("the down weight", *down, format, H, I, a.w2)) return rc;
+    auto row_bytes = [&](int64_t K) { return format == PTB_INT4 ? cdiv<int64_t>(K, kKB) * kInt4BlockBytes : format == dtype ? 2 * K : K; };
+    if (int rc = weight_map(&a.w1.map, gate_up->data, row_bytes(H), I, 2 * E, true)) return rc;
+    if (int rc = weight_map(&a.w2.map, down->data, row_bytes(I), H, E, false)) return rc;
     const int64_t pairs = T * k;
     a.x = x; a.ldx = ldx; a.T = (int) T; a.k = (int) k; a.E = (int) E; a.H = (int) H; a.I = (int) I; a.ids = ids; a.probs = probs; a.out = out;
     const Pieces at = pieces(format, dtype, T, k, H, I);
     uint8_t *ws = (uint8_t *) workspace;
-    a.xs    = scaled_rows_at(ws + at.xs, 1, T, H);
-    a.hs    = scaled_rows_at(ws + at.hs, dtype == PTB_F16 ? 2 : 1, pairs, I);
+    a.xs    = scaled_rows_at(ws + at.xs, T, H);
+    a.hs    = scaled_rows_at(ws + at.hs, pairs, I);
     a.h32   = (float *) (ws + at.hs);
     a.h_hi  = (__nv_bfloat16 *) (ws + at.hs);
     a.h_lo  = a.h_hi + pairs * I;

@@ -130,7 +130,7 @@ def check(rc: int, what: str) -> None:
 # kernel ran out (status codes in include/ptb.h).  Off by default: the check synchronises.
 _DEBUG_STATUS = os.environ.get("PTB_DEBUG_STATUS", "0") not in ("", "0")
 _GEMM_ENTRY_POINTS = ("ptb_gemm_fp8", "ptb_gemm_mxfp8", "ptb_grouped_gemm_fp8", "ptb_grouped_gemm_fp8_variable_k",
-                      "ptb_grouped_gemm_mxfp8", "ptb_grouped_gemm_mxfp8_variable_k")
+                      "ptb_grouped_gemm_mxfp8", "ptb_grouped_gemm_mxfp8_variable_k", "ptb_gemm_int4", "ptb_moe_few_tokens")
 # PTB_NVTX=1: one NVTX range per C-ABI call, named after the entry point (timeline tools show them)
 _NVTX = os.environ.get("PTB_NVTX", "0") not in ("", "0")
 _event_log = None  # when a dict: name -> [(start_event, stop_event), ...] on the launching stream

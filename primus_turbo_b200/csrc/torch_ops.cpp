@@ -1,5 +1,5 @@
 // The eager host path of the public ops: operand checks, allocations, launches and the autograd nodes of
-// gemm_fp8, grouped_gemm_fp8 and the quantise / dequantise ops, in C++ over the C ABI of ptb.h.
+// gemm_fp8, grouped_gemm_fp8, the quantise / dequantise ops, the top-k router and the products of few rows, in C++ over the C ABI of ptb.h.
 //
 // Why native: a small forward (256 x 512 x 1024 blockwise) keeps the GPU busy for 16 us, and the Python form of the
 // same call -- an autograd.Function, a ctypes call and four torch.empty per kernel, a device context each --
@@ -774,10 +774,197 @@ py::object py_dequantize(const Tensor &q, const Tensor &s, ScalarType out_dt, in
     });
 }
 
+// ---- few rows: routing, 4-bit weights, an MoE layer for a few tokens -------------------------------------------------------------
+// Nothing that another layer of torch has wrapped or still watches.
+bool bare(const Tensor &t) {
+    using c10::DispatchKey;
+    return plain_cuda(t) && !t.key_set().has_any(c10::DispatchKeySet({DispatchKey::Python, DispatchKey::PythonTLSSnapshot, DispatchKey::Functionalize,
+                                                                      DispatchKey::FuncTorchBatched, DispatchKey::FuncTorchGradWrapper,
+                                                                      DispatchKey::Batched, DispatchKey::Conjugate, DispatchKey::Negative}));
+}
+bool wants_grad(const Tensor &t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+bool aligned(const Tensor &t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
+// rows of 16-bit values that the kernels read as they are
+bool rows16(const Tensor &x) {
+    return x.dim() == 2 && is_16bit(x.scalar_type()) && x.stride(1) == 1 && aligned(x) && (x.size(0) <= 1 || (x.stride(0) % 8 == 0 && x.stride(0) >= x.size(1)));
+}
+
+// codes [.., ceil(K / 128) * 64], scales [.., ceil(K / group)] and perhaps zero points
+bool int4_parts(const Tensor &q, const Tensor &s, const std::optional<Tensor> &z, const Tensor &beside, int64_t k, int64_t group) {
+    auto fits = [&](const Tensor &t, ScalarType dt) { return bare(t) && t.is_contiguous() && t.device() == beside.device() && t.scalar_type() == dt; };
+    if (group != 32 && group != 64 && group != 128) return false;
+    if (!fits(q, ScalarType::Byte) || !aligned(q) || !fits(s, ScalarType::BFloat16) || (z && !fits(*z, ScalarType::Byte))) return false;
+    return q.size(-1) == cdiv(k, 128) * 64 && s.size(-1) == cdiv(k, group) && (!z || z->sizes() == s.sizes());
+}
+const void *data_or_null(const std::optional<Tensor> &t) { return t ? t->const_data_ptr() : nullptr; }
+
+py::object py_gemm_int4(const Tensor &x_in, const Tensor &q, const Tensor &s, const std::optional<Tensor> &z, int64_t k, int64_t group,
+                        const std::optional<Tensor> &bias) {
+    if (traced() || !bare(x_in) || x_in.dim() < 1 || wants_grad(x_in) || has_tangent(x_in) || x_in.size(-1) != k || q.dim() != 2) return py::none();
+    if (x_in.dim() != 2 && !x_in.is_contiguous()) return py::none();
+    const Tensor x = x_in.dim() == 2 ? x_in : x_in.detach().view({-1, k});
+    const int64_t m = x.size(0), n = q.size(0);
+    if (!rows16(x) || !int4_parts(q, s, z, x, k, group)) return py::none();
+    if (bias && (!bare(*bias) || wants_grad(*bias) || has_tangent(*bias) || bias->dim() != 1 || bias->size(0) != n || !bias->is_contiguous() ||
+                 bias->scalar_type() != x.scalar_type() || bias->device() != x.device()))
+        return py::none();
+    return guarded([&]() -> py::object {
+        Call c(x);
+        auto shape   = x_in.sizes().vec();
+        shape.back() = n;
+        Tensor out = c.empty(shape, x.scalar_type());
+        Tensor ws  = c.empty({ptb_gemm_int4_workspace(code_of(x.scalar_type()), m, k, group)}, ScalarType::Byte);
+        PTB_RUN_GEMM(ptb_gemm_int4, x.const_data_ptr(), code_of(x.scalar_type()), x.stride(0), m, n, k, q.const_data_ptr(), s.const_data_ptr(),
+                     data_or_null(z), group, data_or_null(bias), ws.mutable_data_ptr(), out.mutable_data_ptr(), c.st);
+        return py::cast(out);
+    });
+}
+
+py::object py_quant_int4(const Tensor &w, int64_t group, bool symmetric) {
+    if (traced() || !bare(w) || wants_grad(w) || has_tangent(w) || !is_hp(w.scalar_type()) || !w.is_contiguous() || !aligned(w) || (w.dim() != 2 && w.dim() != 3) ||
+        w.size(-1) % 8 || (group != 32 && group != 64 && group != 128))
+        return py::none();
+    return guarded([&]() -> py::object {
+        Call c(w);
+        auto shape      = w.sizes().vec();
+        const int64_t k = shape.back();
+        shape.back()    = cdiv(k, 128) * 64;
+        Tensor codes    = c.empty(shape, ScalarType::Byte);
+        shape.back()    = cdiv(k, group);
+        Tensor scale = c.empty(shape, ScalarType::BFloat16), zero;
+        if (!symmetric) zero = c.empty(shape, ScalarType::Byte);
+        PTB_RUN(ptb_quant_int4, w.const_data_ptr(), code_of(w.scalar_type()), w.numel() / k, k, group, codes.mutable_data_ptr(), scale.mutable_data_ptr(),
+                symmetric ? nullptr : zero.mutable_data_ptr(), c.st);
+        return py::make_tuple(codes, scale, symmetric ? py::object(py::none()) : py::cast(zero));
+    });
+}
+
+py::object py_dequant_int4(const Tensor &q, const Tensor &s, const std::optional<Tensor> &z, int64_t k, int64_t group, ScalarType dt) {
+    if (traced() || !bare(q) || k < 1 || !is_hp(dt) || !int4_parts(q, s, z, q, k, group)) return py::none();
+    return guarded([&]() -> py::object {
+        Call c(q);
+        auto shape   = q.sizes().vec();
+        shape.back() = k;
+        Tensor out = c.empty(shape, dt);
+        PTB_RUN(ptb_dequant_int4, q.const_data_ptr(), s.const_data_ptr(), data_or_null(z), out.numel() / k, k, group, out.mutable_data_ptr(), code_of(dt), c.st);
+        return py::cast(out);
+    });
+}
+
+// The weights as pytorch/ops/moe/few_tokens.py takes them apart; group > 0: 4-bit.
+py::object py_moe_few_tokens(const Tensor &x, const Tensor &ids, const Tensor &probs, const Tensor &w1, const std::optional<Tensor> &s1,
+                             const std::optional<Tensor> &z1, const Tensor &w2, const std::optional<Tensor> &s2, const std::optional<Tensor> &z2,
+                             int64_t inter, int granularity, int64_t group) {
+    if (traced() || !bare(x) || !bare(ids) || !bare(probs) || !bare(w1) || !bare(w2) || !rows16(x)) return py::none();
+    for (const Tensor *t : {&x, &probs, &w1, &w2})
+        if (wants_grad(*t) || has_tangent(*t)) return py::none();
+    const int64_t T = x.size(0), H = x.size(1);
+    if (ids.dim() != 2 || ids.size(0) != T || ids.scalar_type() != ScalarType::Long || !ids.is_contiguous() || ids.device() != x.device() ||
+        probs.sizes() != ids.sizes() || probs.scalar_type() != ScalarType::Float || !probs.is_contiguous() || probs.device() != x.device())
+        return py::none();
+    const int64_t k = ids.size(1), E = w1.dim() == 3 ? w1.size(0) : 0;
+    if (E < 1 || E > 1024 || w2.dim() != 3 || w2.size(0) != E || w1.size(1) != 2 * inter || w2.size(1) != H || w1.scalar_type() != w2.scalar_type()) return py::none();
+    int format = PTB_INT4;
+    if (group > 0) {
+        if (!s1 || !s2 || !int4_parts(w1, *s1, z1, x, H, group) || !int4_parts(w2, *s2, z2, x, inter, group)) return py::none();
+    } else {
+        format = code_of(w1.scalar_type());
+        auto fits = [&](const Tensor &w, int64_t width, const std::optional<Tensor> &s) {
+            if (w.size(2) != width || !w.is_contiguous() || !aligned(w) || w.device() != x.device()) return false;
+            return format == code_of(x.scalar_type()) ? !s.has_value()
+                                                     : is_fp8(w.scalar_type()) && s && bare(*s) && s->is_contiguous() && s->device() == x.device() &&
+                                                           s->scalar_type() == ScalarType::Float;
+        };
+        if (!fits(w1, H, s1) || !fits(w2, inter, s2)) return py::none();
+    }
+    const int64_t step = is_fp8(w1.scalar_type()) ? 16 : 8;
+    const int64_t need = ptb_moe_few_tokens_workspace(code_of(x.scalar_type()), T, H, inter, k, format);
+    if (need < 0 || H % step || inter % step) return py::none();
+    return guarded([&]() -> py::object {
+        Call c(x);
+        Tensor out = c.empty({T, H}, x.scalar_type()), ws = c.empty({need}, ScalarType::Byte);
+        const PtbExpertWeight a{w1.const_data_ptr(), data_or_null(s1), data_or_null(z1), granularity, (int) group},
+            b{w2.const_data_ptr(), data_or_null(s2), data_or_null(z2), granularity, (int) group};
+        PTB_RUN_GEMM(ptb_moe_few_tokens, x.const_data_ptr(), code_of(x.scalar_type()), x.stride(0), T, H, inter, E, ids.const_data_ptr<int64_t>(),
+                     probs.const_data_ptr<float>(), k, format, &a, &b, ws.mutable_data_ptr(), out.mutable_data_ptr(), c.st);
+        return py::cast(out);
+    });
+}
+
+struct RouterSpec {
+    int64_t k, groups, topk_groups;
+    int score;
+    bool normalize, dense;
+    double scaling;
+};
+// -> (probabilities, routing map or ids), and the ids
+std::pair<Tensor, Tensor> route(const Tensor &l, const std::optional<Tensor> &bias, const RouterSpec &d, Tensor &ids) {
+    Call c(l);
+    const int64_t T = l.size(0), E = l.size(1);
+    ids          = c.empty({T, d.k}, ScalarType::Long);
+    Tensor probs = c.empty({T, d.dense ? E : d.k}, ScalarType::Float), map;
+    if (d.dense) map = c.empty({T, E}, ScalarType::Bool);
+    float *p = probs.mutable_data_ptr<float>();
+    PTB_RUN(ptb_topk_router, l.const_data_ptr(), code_of(l.scalar_type()), T, E, l.stride(0), d.k, d.score, bias ? bias->const_data_ptr<float>() : nullptr,
+            d.groups, d.topk_groups, d.normalize, (float) d.scaling, ids.mutable_data_ptr<int64_t>(), d.dense ? nullptr : p, d.dense ? p : nullptr,
+            d.dense ? map.mutable_data_ptr() : nullptr, c.st);
+    return {probs, d.dense ? map : ids};
+}
+
+struct RouterFn : public torch::autograd::Function<RouterFn> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &logits, const std::optional<Tensor> &bias, const RouterSpec &d) {
+        Tensor ids;
+        auto [probs, chosen] = route(logits, bias, d, ids);
+        ctx->save_for_backward({logits, ids});
+        ctx->mark_non_differentiable({chosen});
+        put(ctx, "spec", (int64_t) d.score | (int64_t) d.normalize << 8 | (int64_t) d.dense << 9);
+        ctx->saved_data["scaling"] = d.scaling;
+        return {probs, chosen};
+    }
+    static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+        TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), "the gradient of topk_router has no derivative of its own (create_graph)");
+        return in_backward([&] {
+            const auto sv = ctx->get_saved_variables();
+            const Tensor &l = sv[0], &ids = sv[1];
+            const int64_t spec = take(ctx, "spec");
+            Tensor g = grads[0].scalar_type() == ScalarType::Float ? grads[0] : grads[0].to(ScalarType::Float);
+            if (g.stride(1) != 1) g = g.contiguous();
+            Call c(l);
+            Tensor out = c.empty(l.sizes(), l.scalar_type());
+            PTB_RUN(ptb_topk_router_bwd, l.const_data_ptr(), code_of(l.scalar_type()), l.size(0), l.size(1), l.stride(0), ids.size(1), (int) (spec & 255),
+                    (int) (spec >> 8 & 1), (float) ctx->saved_data["scaling"].toDouble(), ids.const_data_ptr<int64_t>(), g.const_data_ptr<float>(), g.stride(0),
+                    (int) (spec >> 9 & 1), out.mutable_data_ptr(), c.st);
+            return variable_list{out, Tensor(), Tensor()};
+        });
+    }
+};
+
+py::object py_topk_router(const Tensor &l, const std::optional<Tensor> &bias, int64_t k, int score, int64_t groups, int64_t topk_groups, bool normalize,
+                          double scaling, bool dense) {
+    if (traced() || !bare(l) || has_tangent(l) || l.dim() != 2 || !is_hp(l.scalar_type()) || l.stride(1) != 1 || (l.size(0) > 1 && l.stride(0) < l.size(1)))
+        return py::none();
+    const int64_t E = l.size(1);
+    if (E > 1024 || groups < 1 || groups > 32 || E % groups || topk_groups < 1 || topk_groups > groups || k < 1 || k > 32 || k > E / groups * topk_groups)
+        return py::none();
+    if (bias && (!bare(*bias) || bias->dim() != 1 || bias->size(0) != E || bias->scalar_type() != ScalarType::Float || !bias->is_contiguous() ||
+                 bias->device() != l.device() || has_tangent(*bias)))
+        return py::none();
+    const RouterSpec d{k, groups, topk_groups, score, normalize, dense, scaling};
+    return guarded([&]() -> py::object {
+        if (wants_grad(l)) {
+            const auto out = RouterFn::apply(l, bias, d);
+            return py::make_tuple(out[0], out[1]);
+        }
+        Tensor ids;
+        auto [probs, chosen] = route(l, bias, d, ids);
+        return py::make_tuple(probs, chosen);
+    });
+}
+
 } // namespace
 
 PYBIND11_MODULE(ptb_torch, m) {
-    m.doc() = "native host path of the FP8 ops";
+    m.doc() = "native host path of the FP8 ops, the router, 4-bit weights and the few-token MoE layer";
     m.def("setup", [](py::object error_class, py::object timed_region) {
         g_error_class  = error_class.release().ptr(); // both kept for the life of the process
         g_timed_region = timed_region.release().ptr();
@@ -790,4 +977,9 @@ PYBIND11_MODULE(ptb_torch, m) {
     m.def("quantize", &py_quantize);
     m.def("quantize_dual", &py_quantize_dual);
     m.def("dequantize", &py_dequantize);
+    m.def("gemm_int4", &py_gemm_int4);
+    m.def("quant_int4", &py_quant_int4);
+    m.def("dequant_int4", &py_dequant_int4);
+    m.def("moe_few_tokens", &py_moe_few_tokens);
+    m.def("topk_router", &py_topk_router);
 }

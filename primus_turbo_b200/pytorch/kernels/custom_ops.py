@@ -269,11 +269,13 @@ def _(x, ids, probs, w1, w1_scale, w1_zero, w2, w2_scale, w2_zero, inter, granul
 # this module therefore run the op's own body directly in plain eager mode and go through the registered op
 # only while compiling or under a dispatch mode (FakeTensorMode, functionalisation, ...), where the op and its
 # fake kernel are what the tracer needs.  Same function either way; `.op` is the registered op.
-def _with_eager_fast_path(op):
+def _with_eager_fast_path(op, traceable=False):
+    """``traceable``: an op that no autograd.Function stands around; torch.jit.trace has to see the registered op, since of the
+    body it would record the allocations alone."""
     body = op._init_fn  # the undecorated function the op was created from
 
     def call(*args, **kwargs):
-        if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0:
+        if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0 or (traceable and torch.jit.is_tracing()):
             return op(*args, **kwargs)
         return body(*args, **kwargs)
 
@@ -287,5 +289,5 @@ for _name in ("quantize_fp8_tensorwise", "quantize_fp8_rowwise", "quant_fp8_bloc
               "quant_fp8_blockwise_for_weight", "quant_fp8_blockwise_segment_m_row_col", "dequantize_fp8", "gemm_fp8_impl",
               "grouped_gemm_fp8_impl", "grouped_gemm_fp8_variable_k_impl", "topk_router", "topk_router_bwd", "quant_int4",
               "dequant_int4", "gemm_int4", "moe_few_tokens"):
-    globals()[_name] = _with_eager_fast_path(globals()[_name])
+    globals()[_name] = _with_eager_fast_path(globals()[_name], _name in ("gemm_int4", "moe_few_tokens"))
 del _name

@@ -12,6 +12,7 @@ from typing import Optional
 
 import torch
 
+from primus_turbo_b200 import _native
 from primus_turbo_b200._lib import PtbError, require_cuda
 from primus_turbo_b200.pytorch.core.int4_weight import INT4_GROUP_SIZES, Int4Weight
 from primus_turbo_b200.pytorch.kernels import custom_ops as _ops
@@ -38,6 +39,10 @@ def quantize_int4(w: torch.Tensor, group_size: int = 128, symmetric: bool = True
     ``symmetric``: ``scale = max |w| / 7`` and codes around 8; otherwise the range of a group, 0 included, in 15 steps from a
     zero point.  The scale is rounded to bf16 before the codes are chosen.  A group that holds a NaN or an infinity becomes
     NaN as a whole.  ``w`` is taken as it is: no gradient flows through (pass a detached tensor, or call under ``no_grad``)."""
+    if _native.usable(w):
+        parts = _native.ext.quant_int4(w, group_size, symmetric)
+        if parts is not None:
+            return Int4Weight(*parts, w.shape, group_size)
     refuse_gradient("quantize_int4", w)
     if w.dim() not in (2, 3):
         raise ValueError(f"a 4-bit weight is 2D or 3D, got {w.dim()}D")
@@ -58,6 +63,10 @@ def dequantize_int4(w: Int4Weight, out_dtype: torch.dtype = torch.bfloat16) -> t
         raise TypeError(f"dequantize_int4 takes an Int4Weight, got {type(w).__name__}")
     if out_dtype not in _WIDE:
         raise ValueError(f"dequantize_int4 gives bf16, fp16 or fp32, not {out_dtype}")
+    if _native.usable(w.qdata):
+        out = _native.ext.dequant_int4(w.qdata, w.scale, w.zero, w.shape[-1], w.group_size, out_dtype)
+        if out is not None:
+            return out
     require_cuda(w.qdata)
     return _ops.dequant_int4(w.qdata, w.scale, w.zero, w.shape[-1], w.group_size, out_dtype)
 
@@ -70,6 +79,10 @@ def gemm_int4(x: torch.Tensor, w: Int4Weight, bias: Optional[torch.Tensor] = Non
     library product is the faster way."""
     if not isinstance(w, Int4Weight):
         raise TypeError(f"gemm_int4 takes an Int4Weight, got {type(w).__name__}")
+    if _native.usable(x):
+        y = _native.ext.gemm_int4(x, w.qdata, w.scale, w.zero, w.shape[-1], w.group_size, bias)
+        if y is not None:
+            return y
     refuse_gradient("gemm_int4", x, bias)
     if w.ndim != 2:
         raise ValueError(f"gemm_int4 takes a 2D weight, got {w.ndim}D")

@@ -10,6 +10,7 @@ from typing import Union
 
 import torch
 
+from primus_turbo_b200 import _native
 from primus_turbo_b200._lib import PtbError, require_cuda
 from primus_turbo_b200.pytorch.core.int4_weight import Int4Weight
 from primus_turbo_b200.pytorch.core.low_precision import ScalingGranularity
@@ -51,6 +52,23 @@ def _parts(name: str, w: Weight, dtype: torch.dtype):
     return "raw", w.contiguous(), None, None, 0, 0
 
 
+def _native_layer(x, ids, probs, w1, w2):
+    """The call through the native host path; ``None`` where it has to run in Python."""
+    if type(w1) is Int4Weight and type(w2) is Int4Weight:
+        if len(w1.shape) != 3 or len(w2.shape) != 3 or w1.group_size != w2.group_size or w1.shape[2] != x.shape[-1]:
+            return None
+        return _native.ext.moe_few_tokens(x, ids, probs, w1.qdata, w1.scale, w1.zero, w2.qdata, w2.scale, w2.zero, w2.shape[2], 0, w1.group_size)
+    if isinstance(w1, QuantizedTensor) and isinstance(w2, QuantizedTensor):
+        if w1.requires_grad or w2.requires_grad:
+            return None
+        kind, d1, s1, _, g1, _ = _parts("w_gate_up", w1, x.dtype)
+        _, d2, s2, _, g2, _ = _parts("w_down", w2, x.dtype)
+        return _native.ext.moe_few_tokens(x, ids, probs, d1, s1, None, d2, s2, None, w2.shape[2], g1, 0) if g1 == g2 else None
+    if _native.usable(w1) and _native.usable(w2) and w2.dim() == 3:
+        return _native.ext.moe_few_tokens(x, ids, probs, w1, None, None, w2, None, None, w2.shape[2], 0, 0)
+    return None
+
+
 def moe_few_tokens(
     x: torch.Tensor, topk_ids: torch.Tensor, topk_probs: torch.Tensor, w_gate_up: Weight, w_down: Weight
 ) -> torch.Tensor:
@@ -65,6 +83,10 @@ def moe_few_tokens(
     Activations are not quantised.  Sums are kept in fp32, and the activation between the two products in more than bf16;
     the result is rounded once to x's type.  Equal inputs give equal bits.  Every call allocates its own workspace, so calls on
     several streams or in several captured graphs do not share any."""
+    if _native.usable(x):
+        y = _native_layer(x, topk_ids, topk_probs, w_gate_up, w_down)
+        if y is not None:
+            return y
     refuse_gradient("moe_few_tokens", x, topk_probs, *(w for w in (w_gate_up, w_down) if isinstance(w, torch.Tensor)))
     if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"x must be [tokens, hidden] in bf16 or fp16, got {x.dim()}D {x.dtype}")

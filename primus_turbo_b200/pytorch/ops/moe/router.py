@@ -12,6 +12,7 @@ from typing import Optional, Tuple
 import torch
 from torch.autograd.function import once_differentiable
 
+from primus_turbo_b200 import _native
 from primus_turbo_b200._lib import PtbError, require_cuda
 from primus_turbo_b200.pytorch.kernels import custom_ops as _ops
 from primus_turbo_b200.pytorch.kernels.few_rows_impl import SCORE_FUNCTIONS
@@ -39,6 +40,10 @@ class _TopkRouter(torch.autograd.Function):
 
 
 def _route(logits, topk, score_function, expert_bias, num_groups, topk_groups, normalize, scaling_factor, dense):
+    if _native.usable(logits) and score_function in SCORE_FUNCTIONS:
+        out = _native.ext.topk_router(logits, expert_bias, topk, SCORE_FUNCTIONS[score_function], num_groups, topk_groups, normalize, scaling_factor, dense)
+        if out is not None:
+            return out
     if logits.dim() != 2:
         raise ValueError(f"logits must be [tokens, experts], got {logits.dim()}D")
     if logits.dtype not in (torch.float32, torch.float16, torch.bfloat16):

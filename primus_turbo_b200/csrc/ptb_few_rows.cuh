@@ -289,6 +289,18 @@ template <int FMT, int G> struct BlockScale {
     // the row's scales of block kb; zeros where there are none (there x and the codes are zero)
     __device__ __forceinline__ void load(const RowScale<FMT> &r, int kb, int blocks) {
         if constexpr (FMT == kWInt4) {
+            if (kN > 1 && kb * kN + kN <= r.count && reinterpret_cast<uintptr_t>(r.s4 + kb * kN) % (2 * kN) == 0 && (r.z4 == nullptr || reinterpret_cast<uintptr_t>(r.z4 + kb * kN) % kN == 0)) {
+                if constexpr (kN == 4) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(r.s4 + kb * kN);
+                    s[0] = v.x;
+                    s[kWords - 1] = v.y;
+                    z = r.z4 != nullptr ? *reinterpret_cast<const uint32_t *>(r.z4 + kb * kN) : 0x08080808u;
+                } else {
+                    s[0] = *reinterpret_cast<const uint32_t *>(r.s4 + kb * kN);
+                    z    = r.z4 != nullptr ? *reinterpret_cast<const uint16_t *>(r.z4 + kb * kN) : 0x0808u;
+                }
+                return;
+            }
             z = 0;
 #pragma unroll
             for (int i = 0; i < kN; ++i) {
@@ -455,18 +467,22 @@ template <typename T, int FMT, int G, int FL, int NT, int WR, int kTerms, bool k
 __device__ __forceinline__ void few_rows_walk(float (&acc)[NT][4], uint8_t *smem, uint64_t *bars, const CUtensorMap *map, int K, int cols, int begin, int end, const Src &src) {
     using W = Walk<FMT, NT, WR>;
     using Piece = RowPiece<FMT>;
-    constexpr int CB = kChunk<FMT>, kXPasses = (kTerms * NT * 8 + 31) / 32;
+    constexpr int CB = kChunk<FMT>;
+    constexpr bool kMerge = NT <= 4; // the two blocks of a pair as one piece of code: more to do while something is waited for, but more registers
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int blocks = (K + kKB - 1) / kKB, live = (cols + 7) / 8, x_rows = kTerms * cols;
+    const int live = (cols + 7) / 8, x_rows = kTerms * cols, x_warps = (x_rows + 7) / 8;
     const uint32_t ring = shared_u32(smem) + warp * (kWeightSlots * kSlotBytes), x_ring = shared_u32(smem) + WR * (kWeightSlots * kSlotBytes), x_stage = x_rows * kXPitch;
     const uint32_t w_bars = shared_u32(bars) + warp * (kWeightSlots * 8), x_bars = shared_u32(bars) + WR * (kWeightSlots * 8), read_bars = x_bars + 2 * 8;
-    if (threadIdx.x < W::kBars) bar_init(shared_u32(bars) + threadIdx.x * 8, threadIdx.x < W::kBars - 2 ? 1 : WR);
+    if (threadIdx.x < W::kBars) bar_init(shared_u32(bars) + threadIdx.x * 8, (int) threadIdx.x < WR * kWeightSlots ? 1 : threadIdx.x < W::kBars - 2 ? x_warps : WR);
     bar_init_fence();
     __syncthreads();
 
+    // Whole pairs are read: where the last has one block, the other is zeros.
+    const int pairs = (end - begin + kPair - 1) / kPair;
     int kb_w = begin;
     auto fetch_weights = [&](int slot) {
-        if (kb_w < end && lane == 0) fetch_tile<FMT>(ring + slot * kSlotBytes, map, kb_w, min(CB, end - kb_w), src.row, src.slab, w_bars + slot * 8);
+        if (kb_w < begin + pairs * kPair && lane == 0)
+            fetch_tile<FMT>(ring + slot * kSlotBytes, map, kb_w, min(CB, begin + pairs * kPair - kb_w), src.row, src.slab, w_bars + slot * 8);
         kb_w += CB;
     };
     BlockScale<FMT, G> next[2], mine[2];
@@ -476,96 +492,100 @@ __device__ __forceinline__ void few_rows_walk(float (&acc)[NT][4], uint8_t *smem
     for (int i = 0; i < kWeightSlots; ++i) fetch_weights(i);
     grid_dep_wait();
     grid_dep_open();
-    const uint8_t *xp[kXPasses];
-#pragma unroll
-    for (int i = 0; i < kXPasses; ++i) {
-        const int row = min(lane + 32 * i, x_rows - 1), term = kTerms > 1 && row >= cols ? 1 : 0;
-        xp[i] = src.x(term, row - term * cols);
-    }
-    auto fetch_x = [&](int kb, int stage) { // by one warp
-        const int n = min(kPair, end - kb);
-        uint32_t bytes = n * W::kXStep;
-        const uint32_t to = x_ring + stage * x_stage;
-        if (!kScaledX<FMT> && (kb + n) * kKB > K) { // zeros behind the end: the weights are zero there too, but what lies here might be a NaN
-            bytes = (K - kb * kKB) * 2;
-            for (int i = lane; i < x_rows * (kPair * 16); i += 32)
-                if ((i % (kPair * 16)) * 16 >= bytes) zero16(to + i / (kPair * 16) * kXPitch + (i % (kPair * 16)) * 16);
-            __syncwarp();
-        }
-        if (lane == 0) bar_expect(x_bars + stage * 8, x_rows * bytes);
+    // By the warps in turn, eight rows each: a copy takes a warp some 60 clocks.
+    auto fetch_x = [&](int pair, auto &&free) {
+        const int turn = (warp - pair) & (WR - 1), row = turn * 8 + lane, kb = begin + pair * kPair, stage = pair & 1;
+        if (turn >= x_warps || !free()) return;
+        uint32_t bytes = kScaledX<FMT> ? min(kPair, end - kb) * kScaledBlock : min(kPair * kKB, K - kb * kKB) * 2;
+        const uint32_t to = x_ring + stage * x_stage + row * kXPitch;
+        const bool mine = lane < 8 && row < x_rows;
+        if (mine) // zeros behind the end: the weights are zero there too, but what lies here might be a NaN
+            for (uint32_t i = bytes; i < kPair * W::kXStep; i += 16) zero16(to + i);
         __syncwarp();
-#pragma unroll
-        for (int i = 0; i < kXPasses; ++i)
-            if (lane + 32 * i < x_rows) bulk_copy(to + (lane + 32 * i) * kXPitch, xp[i] + (int64_t) kb * W::kXStep, bytes, x_bars + stage * 8);
+        if (lane == 0) bar_expect(x_bars + stage * 8, min(8, x_rows - turn * 8) * bytes);
+        __syncwarp();
+        if (mine) {
+            const int term = kTerms > 1 && row >= cols ? 1 : 0;
+            bulk_copy(to, src.x(term, row - term * cols) + (int64_t) kb * W::kXStep, bytes, x_bars + stage * 8);
+        }
     };
-    if (warp < 2 && begin + warp * kPair < end) fetch_x(begin + warp * kPair, warp);
+#pragma unroll 1
+    for (int i = 0; i < 2 && i < pairs; ++i) fetch_x(i, [] { return true; });
 
     const uint32_t w_lane = ring + lane_place();
     const uint32_t x_lane = x_ring + g * kXPitch + t * 16, run_lane = x_ring + 2 * t * kXPitch + 256, term_bytes = cols * kXPitch;
-    int slot = 0, in = 0; // in: blocks done of the chunk
-    uint32_t w_parity = 0, x_at = 0, w_at = 0;
+    int slot = 0;
+    uint32_t w_parity = 0;
     bool ok = true;
+    auto next_chunk = [&] {
+        if (ok) ok = __all_sync(0xffffffffu, bar_wait(w_bars + slot * 8, w_parity));
+    };
+    auto chunk_read = [&] {
+        __syncwarp();
+        if (ok) fetch_weights(slot);
+        if (++slot == kWeightSlots) { slot = 0; w_parity ^= 1; }
+    };
 #pragma unroll 1
-    for (int kb = begin; kb < end; ++kb) {
+    for (int pair = 0; pair < pairs; ++pair) {
+        const int kb = begin + pair * kPair, stage = pair & 1, in = kb % CB; // in: blocks done of the chunk
         if (in == 0) {
-            if (ok) ok = __all_sync(0xffffffffu, bar_wait(w_bars + slot * 8, w_parity));
-            w_at = w_lane + slot * kSlotBytes;
+            next_chunk();
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 mine[h] = next[h];
                 next[h].load(src.scale[h], kb + CB + t, end);
             }
         }
-        const int pair = (kb - begin) / kPair, stage = pair & 1;
-        const bool first = (kb - begin) % kPair == 0;
-        if (first) {
-            if (ok) ok = __all_sync(0xffffffffu, bar_wait(x_bars + stage * 8, pair >> 1 & 1));
-            x_at = stage * x_stage;
-        }
+        if (ok) ok = __all_sync(0xffffffffu, bar_wait(x_bars + stage * 8, pair >> 1 & 1));
+        auto refill = [&] { // the pair after this one
+            if (pair > 0 && pair + 1 < pairs)
+                fetch_x(pair + 1, [&] {
+                    if (ok) ok = __all_sync(0xffffffffu, bar_wait(read_bars + (stage ^ 1) * 8, (pair - 1) >> 1 & 1));
+                    return ok;
+                });
+        };
+        if (kMerge) refill();
         if (ok) {
-            Piece p[2];
-            p[0].read(w_at, in, 0);
-            p[1].read(w_at, in, 8 * 128);
-            auto x = [&](int i, int term, int q) { return read16(x_lane + x_at + i * (8 * kXPitch) + term * term_bytes + q * 64); };
-            BlockScale<FMT, G> s[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) s[h] = mine[h].from_lane((lane & 28) | in);
+            const uint32_t x_at = stage * x_stage;
             by_live<NT>(live, [&](auto n) {
                 constexpr int N = decltype(n)::value;
-                if constexpr (kScaledX<FMT>) {
-                    half_block<FMT, G, FL, N, kTerms>(acc, p, s, src.scale[0].z4 != nullptr, x, [&](int i, int f, int c) { return read4(run_lane + x_at + (i * 8 + c) * kXPitch + f * 4); });
-                } else if constexpr (!kSplit) {
-                    word_block<T, N, kTerms>(acc, p[0], p[1], x);
-                } else { // fp16 weights become the sum of two bf16, exactly
-                    Piece ha, hb, la, lb;
-                    split_half(p[0], ha, la);
-                    split_half(p[1], hb, lb);
-                    word_block<T, N, kTerms>(acc, ha, hb, x);
-                    word_block<T, N, 1>(acc, la, lb, x);
+#pragma unroll(kMerge ? kPair : 1)
+                for (int u = 0; u < kPair; ++u) {
+                    if (!kMerge && u > 0) refill();
+                    if (CB == 1 && u > 0) {
+                        chunk_read();
+                        next_chunk();
+                    }
+                    Piece p[2];
+                    p[0].read(w_lane + slot * kSlotBytes, CB > kPair ? in + u : CB > 1 ? u : 0, 0);
+                    p[1].read(w_lane + slot * kSlotBytes, CB > kPair ? in + u : CB > 1 ? u : 0, 8 * 128);
+                    auto x = [&](int i, int term, int q) { return read16(x_lane + x_at + u * W::kXStep + i * (8 * kXPitch) + term * term_bytes + q * 64); };
+                    if constexpr (kScaledX<FMT>) {
+                        BlockScale<FMT, G> s[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) s[h] = mine[h].from_lane((lane & 28) | (CB > kPair ? in + u : u));
+                        half_block<FMT, G, FL, N, kTerms>(acc, p, s, src.scale[0].z4 != nullptr, x,
+                                                          [&](int i, int f, int c) { return read4(run_lane + x_at + u * W::kXStep + (i * 8 + c) * kXPitch + f * 4); });
+                    } else if constexpr (!kSplit) {
+                        word_block<T, N, kTerms>(acc, p[0], p[1], x);
+                    } else { // fp16 weights become the sum of two bf16, exactly
+                        Piece ha, hb, la, lb;
+                        split_half(p[0], ha, la);
+                        split_half(p[1], hb, lb);
+                        word_block<T, N, kTerms>(acc, ha, hb, x);
+                        word_block<T, N, 1>(acc, la, lb, x);
+                    }
                 }
             });
         }
-        if (++in == CB || kb == end - 1) {
-            __syncwarp();
-            if (ok) fetch_weights(slot);
-            in = 0;
-            if (++slot == kWeightSlots) { slot = 0; w_parity ^= 1; }
-        }
-        x_at += W::kXStep;
-        if (!first || kb == end - 1) {
-            __syncwarp();
-            if (lane == 0) bar_arrive(read_bars + stage * 8);
-        }
-        if (first && pair > 0 && kb + kPair < end && warp == pair % WR) {
-            if (ok) ok = __all_sync(0xffffffffu, bar_wait(read_bars + (stage ^ 1) * 8, (pair - 1) >> 1 & 1));
-            if (ok) fetch_x(kb + kPair, stage ^ 1);
-        }
+        if (in + kPair >= CB || pair == pairs - 1) chunk_read();
+        __syncwarp();
+        if (lane == 0) bar_arrive(read_bars + stage * 8);
     }
     if (!ok) { // the result is incomplete; what is on its way lands before the CTA gives its memory back
         if (lane == 0) atomicExch(&g_few_status, 5);
         for (int i = 0; i < kWeightSlots; ++i) bar_wait(w_bars + i * 8, i < slot ? w_parity ^ 1 : w_parity);
-        const int last = (end - 1 - begin) / kPair;
-        for (int i = max(last - 1, 0); i <= last; ++i) bar_wait(x_bars + (i & 1) * 8, i >> 1 & 1);
+        for (int i = max(pairs - 2, 0); i < pairs; ++i) bar_wait(x_bars + (i & 1) * 8, i >> 1 & 1);
     }
     __syncthreads();
     if (threadIdx.x < W::kBars) bar_end(shared_u32(bars) + threadIdx.x * 8);

@@ -343,8 +343,7 @@ template <int FMT, int G, int FL, int NT, int kTerms, int kMost, typename X, typ
 __device__ __forceinline__ void half_block(float (&acc)[kMost][4], const RowPiece<FMT> (&p)[2], const BlockScale<FMT, G> (&s)[2], bool zeros, X &&x, R &&scale) {
     static_assert(FL == 64 || FL == 128, "an octet of 8-bit weights covers 64 neighbouring k");
     constexpr int kRun = G < FL ? G : FL;
-    constexpr bool kBetween = kRun < FL && NT <= 4; // sums over the groups of a run: registers for a multiplication
-    float c[NT][4], b[kBetween ? NT : 1][4];
+    float c[NT][4], b[NT][4];
     uint32_t za[2] = {0xe408e408u, 0xe408e408u}, zb[2] = {0xd480d480u, 0xd480d480u}; // of zero points of 8
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -370,17 +369,12 @@ __device__ __forceinline__ void half_block(float (&acc)[kMost][4], const RowPiec
         if (!end) continue;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-            if constexpr (kBetween) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) b[i][j] = first ? c[i][j] * w[j >> 1] : b[i][j] + c[i][j] * w[j >> 1];
-                if (!last) continue;
-            }
+            for (int j = 0; j < 4; ++j) b[i][j] = first ? c[i][j] * w[j >> 1] : b[i][j] + c[i][j] * w[j >> 1];
+            if (!last) continue;
             const float xs[2] = {scale(i, q / (FL / 32), 0), scale(i, q / (FL / 32), 1)};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if constexpr (kBetween) acc[i][j] += b[i][j] * xs[j & 1];
-                else acc[i][j] += c[i][j] * w[j >> 1] * xs[j & 1];
-            }
+            for (int j = 0; j < 4; ++j) acc[i][j] += b[i][j] * xs[j & 1];
         }
     }
 }
@@ -431,9 +425,9 @@ template <int FMT, int NT, int WR> struct Walk {
     static constexpr int kXStep = kScaledX<FMT> ? kScaledBlock : 256;
     static constexpr int kBars = WR * kWeightSlots + 2 * kPair;
     static constexpr int kSums = NT * 8 * (kRows + 1) * 4;
-    // what the CTA's shared memory has to hold: the slots and the ring, read past its end by what by_live adds, then the sums and `more`
+    // what the CTA's shared memory has to hold: the slots and the ring, read to the end of eight columns, then the sums and `more`
     static int smem(int terms, int cols, int more = 0) {
-        const int a = WR * kWeightSlots * kSlotBytes + (2 * terms * cols + (NT > 4 ? 15 : 7)) * kXPitch, b = kSums + more;
+        const int a = WR * kWeightSlots * kSlotBytes + (2 * terms * cols + 7) * kXPitch, b = kSums + more;
         return (a > b ? a : b) + kAlign;
     }
 };
@@ -451,11 +445,10 @@ template <int FMT> __device__ __forceinline__ void fetch_tile(uint32_t slot, con
     if (boxes > 1) box_copy(slot + kBoxBytes, map, kb * kBytes + 128, row, slab, bar);
 }
 
-// body(the number of eights of x as a constant, or one more): branches on it in the middle of a block cost ten instructions each.
+// body(the number of eights of x as a constant): branches on it in the middle of a block cost ten instructions each.
 template <int NT, typename F> __device__ __forceinline__ void by_live(int live, F &&body) {
-    constexpr int kLess = NT > 4 ? NT - 2 : NT - 1;
-    if constexpr (kLess > 0)
-        if (live <= kLess) return by_live<kLess>(live, body);
+    if constexpr (NT > 1)
+        if (live < NT) return by_live<NT - 1>(live, body);
     body(std::integral_constant<int, NT>{});
 }
 
@@ -468,7 +461,6 @@ __device__ __forceinline__ void few_rows_walk(float (&acc)[NT][4], uint8_t *smem
     using W = Walk<FMT, NT, WR>;
     using Piece = RowPiece<FMT>;
     constexpr int CB = kChunk<FMT>;
-    constexpr bool kMerge = NT <= 4; // the two blocks of a pair as one piece of code: more to do while something is waited for, but more registers
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int live = (cols + 7) / 8, x_rows = kTerms * cols, x_warps = (x_rows + 7) / 8;
     const uint32_t ring = shared_u32(smem) + warp * (kWeightSlots * kSlotBytes), x_ring = shared_u32(smem) + WR * (kWeightSlots * kSlotBytes), x_stage = x_rows * kXPitch;
@@ -537,21 +529,17 @@ __device__ __forceinline__ void few_rows_walk(float (&acc)[NT][4], uint8_t *smem
             }
         }
         if (ok) ok = __all_sync(0xffffffffu, bar_wait(x_bars + stage * 8, pair >> 1 & 1));
-        auto refill = [&] { // the pair after this one
-            if (pair > 0 && pair + 1 < pairs)
-                fetch_x(pair + 1, [&] {
-                    if (ok) ok = __all_sync(0xffffffffu, bar_wait(read_bars + (stage ^ 1) * 8, (pair - 1) >> 1 & 1));
-                    return ok;
-                });
-        };
-        if (kMerge) refill();
+        if (pair > 0 && pair + 1 < pairs) // the pair after this one
+            fetch_x(pair + 1, [&] {
+                if (ok) ok = __all_sync(0xffffffffu, bar_wait(read_bars + (stage ^ 1) * 8, (pair - 1) >> 1 & 1));
+                return ok;
+            });
         if (ok) {
             const uint32_t x_at = stage * x_stage;
             by_live<NT>(live, [&](auto n) {
                 constexpr int N = decltype(n)::value;
-#pragma unroll(kMerge ? kPair : 1)
+#pragma unroll // (one piece of code: more to do while something is waited for)
                 for (int u = 0; u < kPair; ++u) {
-                    if (!kMerge && u > 0) refill();
                     if (CB == 1 && u > 0) {
                         chunk_read();
                         next_chunk();

@@ -264,8 +264,10 @@ template <typename T, int G> __global__ void __launch_bounds__(32 * kTokenWarps,
         });
 }
 
-// More rows: a CTA has WR * 16 weight rows and up to NT * 8 rows of x.  The CTAs of a cluster share k; each adds up, and writes, its part of the
-// results, in the order of k.
+// More rows: a CTA has WR * 16 weight rows and up to NT * 8 rows of x, at most 32; more rows are shared out among more CTAs, which then read the weight
+// again, mostly from L2.  (64 rows a CTA, with 16 warps: 47 instead of 49 us at 8192 x 8192, but 88 instead of 44 at 4096 x 14336 and
+// 17 instead of 8 at 1024 x 512, for want of CTAs.)  Up to 16 rows four warps, beyond eight: 9 rows, 5760 x 2880, groups of 128: 11 us with four
+// and 12 with eight; 24 rows, 14336 x 4096: 35 and 25.  The CTAs of a cluster share k; each adds up, and writes, its part of the results, in the order of k.
 template <int G> struct Int4BatchRows : Int4Rows<G> {
     ScaledRows xs;
     int row0;
@@ -283,13 +285,13 @@ __device__ __forceinline__ float read_peer(const float *p, uint32_t rank) {
     return v;
 }
 template <typename T, int G, int NT, int WR>
-__global__ void __launch_bounds__(32 * WR, 16 / WR) int4_gemm_kernel(const __grid_constant__ Int4GemmArgs a, int shares) {
+__global__ void __launch_bounds__(32 * WR, 16 / WR) int4_gemm_kernel(const __grid_constant__ Int4GemmArgs a, int shares, int per) {
     extern __shared__ __align__(16) uint8_t raw[];
     uint8_t *smem = aligned(raw);
     using W = Walk<kWInt4, NT, WR>;
     __shared__ uint64_t bars[W::kBars];
     const int tile = blockIdx.x / shares, share = blockIdx.x % shares; // (the rank in the cluster)
-    const int n0 = tile * W::kRows, m0 = blockIdx.y * (NT * 8), cols = min(NT * 8, a.M - m0);
+    const int n0 = tile * W::kRows, m0 = blockIdx.y * per, cols = min(per, a.M - m0);
     const int blocks = (a.K + kKB - 1) / kKB, chunks = (blocks + kChunk<kWInt4> - 1) / kChunk<kWInt4>;
     Int4BatchRows<G> src;
     src.aim(a, n0 + (threadIdx.x >> 5) * 16);
@@ -316,11 +318,12 @@ template <typename T, int G, int NT, int WR> int launch_tile(const Int4GemmArgs 
     using W = Walk<kWInt4, NT, WR>;
     int sms = 0;
     if (int rc = sm_count(&sms)) return rc;
-    const int tiles = cdiv(a.N, W::kRows), sets = cdiv(a.M, NT * 8), chunks = cdiv(a.K, kKB * kChunk<kWInt4>);
+    const int per = cdiv(cdiv(a.M, cdiv(a.M, NT * 8)), 8) * 8, sets = cdiv(a.M, per); // rows of x a CTA, eights as even as can be
+    const int tiles = cdiv(a.N, W::kRows), chunks = cdiv(a.K, kKB * kChunk<kWInt4>);
     int shares = 1; // of k: as many as it takes to give every SM its 16 warps
     while (shares < 8 && 2 * shares <= chunks && (int64_t) tiles * sets * shares * 2 <= (int64_t) sms * (16 / WR)) shares *= 2;
     PTB_CUDA(launch_early(int4_gemm_kernel<T, G, NT, WR>, dim3((unsigned) (tiles * shares), (unsigned) sets), W::kThreads,
-                          (size_t) W::smem(1, (int) imin(a.M, NT * 8)), st, (unsigned) shares, a, shares));
+                          (size_t) W::smem(1, (int) imin(a.M, per)), st, (unsigned) shares, a, shares, per));
     PTB_LAUNCH_CHECK("int4_gemm_kernel");
     return 0;
 }
@@ -342,7 +345,7 @@ template <typename T, int G> int launch_gemm(const Int4GemmArgs &a, cudaStream_t
     PTB_LAUNCH_CHECK("scale_rows_kernel");
     if (a.M <= 8) return launch_tile<T, G, 1, 4>(a, st);
     if (a.M <= 16) return launch_tile<T, G, 2, 4>(a, st);
-    return a.M <= 32 ? launch_tile<T, G, 4, 8>(a, st) : launch_tile<T, G, 8, 16>(a, st);
+    return launch_tile<T, G, 4, 8>(a, st);
 }
 
 bool is_group(int64_t g) { return g == 32 || g == 64 || g == 128; }

@@ -477,8 +477,8 @@ int ptb_dequant_int4(const void *codes, const void *scale, const void *zero, int
                      void *out, int out_dtype, ptb_stream_t stream);
 /* out[m, n] = sum_k x[m, k] * value[n, k] (+ bias[n]), accumulated in fp32; x [M, K] with rows ldx apart (a multiple of 8
  * where M > 1, 16-byte aligned), bias [N] and out [M, N] in x's type (bf16 or fp16).  Made for few rows; more are taken 32 at a time,
- * each time with another read of the weight.  workspace: 16-byte aligned, of ptb_gemm_int4_workspace bytes.  A row of x that holds a NaN or
- * an infinity gives NaN. */
+ * each time with another read of the weight.  workspace: 16-byte aligned, of ptb_gemm_int4_workspace bytes; calls that may overlap need
+ * one each.  A row of x that holds a NaN or an infinity gives NaN and infinities. */
 int64_t ptb_gemm_int4_workspace(int dtype, int64_t M, int64_t K, int64_t group);
 int ptb_gemm_int4(const void *x, int dtype, int64_t ldx, int64_t M, int64_t N, int64_t K, const void *codes,
                   const void *scale, const void *zero, int64_t group, const void *bias, void *workspace, void *out,
@@ -488,7 +488,7 @@ int ptb_gemm_int4(const void *x, int dtype, int64_t ldx, int64_t M, int64_t N, i
 /* out[t] = sum_j probs[t, j] * W2[e] (silu(u[:I]) * u[I:]), u = W1[e] x[t], e = ids[t, j], for W1 [E, 2 I, H] (gate rows first)
  * and W2 [E, H, I].  x [T, H] bf16 or fp16, rows ldx apart; ids [T, k] int64 and probs [T, k] fp32, contiguous; an id outside
  * [0, E) contributes nothing.  out [T, H] in x's type, contiguous.  Sums are kept in fp32, the activation between the two products
- * in two bf16 parts; equal inputs give equal bits.
+ * in fp16 or 16-bit integers scaled per 64 or 128 channels, with 16-bit weights or fp16 results in two parts; equal inputs give equal bits.
  * format: x's own type code, PTB_E4M3, PTB_E5M2 or PTB_INT4, the same for both weights.  Data contiguous, 16-byte aligned.
  *   FP8: scale holds fp32 inverse scales, by granularity: PTB_TENSORWISE one, PTB_ROWWISE [E, rows], PTB_BLOCKWISE
  *        [E, ceil(rows / 128), ceil(K / 128)].  H and I multiples of 16.

@@ -3,9 +3,9 @@
 //
 // Such a product reads the weight once and does little with it, so it is bound by HBM, and everything here serves to have
 // many wide loads in flight and few instructions per weight.  The weight takes the 16-row side of mma.sync and eight rows of x the
-// other: tcgen05 wants 128 weight rows and its operands in shared memory, which at one to sixteen rows buys nothing but a copy.  A warp
-// walks 128-wide blocks of k.  Weights travel by cp.async into shared-memory slots that belong to the lane that will feed them to the
-// MMA, several blocks ahead, without holding registers and without a barrier: a lane reads back what it copied itself.
+// other: tcgen05 wants 128 weight rows and its operands in shared memory, unpacked, which at one to sixteen rows buys nothing but a copy.  A
+// warp walks 128-wide blocks of k; its weights come as tensor boxes into two slots of its own, which it fills again as soon as it has
+// read them.  No barrier of the CTA stands in the walk.
 //
 // What an MMA is fed with.  Measured on a B200, an SM issues an m16n8k16 of 16-bit floats or an m16n8k32 of bytes every 2.1 clocks (FP8
 // ones are taken apart into these: 5.6), and integer and conversion instructions at 64 lanes a clock; HBM brings 23 bytes a clock
@@ -14,15 +14,17 @@
 //     integer per value, scaled by a power of two per block that brings the largest of its 128 to 2^14 .. 2^15, as a signed high byte
 //     and an unsigned low one.  bf16's eight bits are exact in it down to 2^-7 of the largest; below, a value is off by up to 2^-15 of
 //     the largest.  Sums of a group are exact integers, and scaling them is what costs: with more columns of x than eight it is too much;
-//   * for more (few_rows_walk) codes become fp16 less their zero, exactly, 9 instructions for 8;
+//   * for more (few_rows_walk) codes become fp16 less their zero, exactly, 9 instructions for 8.  That is what bounds it: 48 tokens through 32
+//     experts of 7168 x 2048, groups of 32, 357 us where the weights' 790 MB are 121, with two thirds of all issue slots used.  Of these, scaling
+//     the sums of the groups and their MMAs are a fifth, unpacking an eighth, fetching scales a tenth;
 //   * FP8 weights are converted to fp16, exactly, one instruction for two;
 //   * x goes with fp16 weights as fp16, scaled by a power of two per block into its range, where bf16 and fp16 values are exact down
 //     to 2^-27 of the block's largest;
 //   * 16-bit weights go in with 16-bit x as they are.
 //
-// The order of k inside an MMA is free as long as both operands agree on it.  Lane (g, t) = (lane / 4, lane % 4) of a warp supplies weight
-// rows g and g + 8 and row g of x.  An "octet" is eight neighbouring k of a lane: one MMA of bytes, or two of 16 bits.  A block of
-// 128 is four octets a lane.  Where octet q of lane t lies:
+// The order of k inside an MMA is free as long as both operands agree on it.  Lane (g, t) = (lane / 4, lane % 4) of a warp supplies two weight
+// rows (lane_row() and the eighth after it) and row g of x.  An "octet" is eight neighbouring k of a lane: one MMA of bytes, or two of 16
+// bits.  A block of 128 is four octets a lane.  Where octet q of lane t lies:
 //   16-bit and 4-bit weights  k = 32 q + 8 t                    (octet q of all four lanes: 32 neighbouring k, the smallest 4-bit group)
 //   8-bit weights             k = 64 (q / 2) + 16 t + 8 (q % 2) (16 bytes a lane and load; octets 2 c and 2 c + 1: 64 neighbouring k)
 #pragma once
@@ -183,7 +185,6 @@ __device__ __forceinline__ void block_scale(float largest, int top, float &scale
     inv   = __uint_as_float((uint32_t) (254 + top - e) << 23);
 }
 constexpr int kTopInt = 14, kTopHalf = 13;
-__device__ __forceinline__ int fixed16(float v) { return max(min(__float2int_rn(v), 32767), -32768); }
 // Where value k of a block stands: among the bytes that go with byte codes (lane t's four octets are 32 neighbouring bytes), and among the
 // fp16 of the walk over rows (octet q of the four lanes: 64 neighbouring bytes; with 4-bit weights an octet's order is 0 2 1 3 4 6 5 7).
 __host__ __device__ __forceinline__ int byte_place(int k) { return (k / 8 % 4) * 32 + (k / 32) * 8 + k % 8; }

@@ -4,9 +4,10 @@
 // rows over all of k -- for the down projection of an MoE layer the experts' k one after the other ("segments").  A CTA has one
 // tile or up to 16; 16 warps or down to one share a tile's blocks of k, each a run of neighbouring blocks, and add up at the end in a fixed order.
 //
-// Weights come as bulk copies of 256 bytes a row into slots of the warp's own: no lane computes addresses for them, and they do not queue with
-// the loads from shared memory (as cp.async they did: an FP8 layer took 88 us, which was 46 of computing plus 42 of copying).  Two
-// slots of 4 KB a warp keep 64 to 128 KB an SM on their way, where 23 bytes a clock and a latency of some 1000 clocks need about 25.
+// Weights come as boxes of 16 rows and 256 bytes into slots of the warp's own: one thread asks for them, and they do not queue with
+// the loads from shared memory (as cp.async they did: an FP8 layer took 88 us, which was 46 of computing plus 42 of copying; row by row as bulk copies
+// 82; as boxes 63, where the weights are 54).  Two slots of 4 KB a warp keep 64 to 128 KB an SM on their way, where 23 bytes a clock and a
+// latency of some 1000 clocks need about 25.
 //
 // What bounds it then is instructions: a block of 16 rows (1 KB of 4-bit codes) has 44 clocks of an SM, 176 issue slots.  A scale per group
 // and row would be most of them, if the sums of a group had to be scaled before the next group may be added.  With one token

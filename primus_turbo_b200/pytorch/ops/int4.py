@@ -39,8 +39,8 @@ def quantize_int4(w: torch.Tensor, group_size: int = 128, symmetric: bool = True
     ``symmetric``: ``scale = max |w| / 7`` and codes around 8; otherwise the range of a group, 0 included, in 15 steps from a
     zero point.  The scale is rounded to bf16 before the codes are chosen.  A group that holds a NaN or an infinity becomes
     NaN as a whole.  ``w`` is taken as it is: no gradient flows through (pass a detached tensor, or call under ``no_grad``)."""
-    if _native.usable(w):
-        parts = _native.ext.quant_int4(w, group_size, symmetric)
+    if _native.usable(w) and type(group_size) is int:
+        parts = _native.ext.quant_int4(w, group_size, bool(symmetric))
         if parts is not None:
             return Int4Weight(*parts, w.shape, group_size)
     refuse_gradient("quantize_int4", w)
@@ -75,8 +75,8 @@ def gemm_int4(x: torch.Tensor, w: Int4Weight, bias: Optional[torch.Tensor] = Non
     """``x @ dequantised(w).T (+ bias)`` for ``x`` [..., K] (bf16 or fp16) and a 4-bit weight [N, K]; result [..., N] in x's type.
 
     The activations stay in 16 bits and sums in fp32; the weight is never written out.  Made for few rows (a token, a decoding
-    batch): beyond some dozens of rows the weight is read more than once, and ``dequantize_int4`` with a
-    library product is the faster way."""
+    batch): 32 rows are taken at a time, and beyond some hundreds ``dequantize_int4`` with a library product is the faster way.  A row
+    of ``x`` that holds a NaN or an infinity gives NaN and infinities, other rows are not touched by it."""
     if not isinstance(w, Int4Weight):
         raise TypeError(f"gemm_int4 takes an Int4Weight, got {type(w).__name__}")
     if _native.usable(x):

@@ -1,6 +1,6 @@
 """``moe_few_tokens``: the whole feed-forward part of an MoE layer for a handful of tokens, straight from the weights a model is
 kept in.  What ``token_permute``, two grouped GEMMs, ``swiglu_with_probs`` and ``token_unpermute`` do for a training batch costs a
-decoding step more in launches and row padding than its weights take to read; here it is three kernels that read the
+decoding step more in launches and row padding than its weights take to read; here it is two kernels (a token or a few) or four that read the
 experts that are hit once.  For inference: there is no backward pass.  The reference has no counterpart.
 """
 

@@ -40,8 +40,9 @@ class _TopkRouter(torch.autograd.Function):
 
 
 def _route(logits, topk, score_function, expert_bias, num_groups, topk_groups, normalize, scaling_factor, dense):
-    if _native.usable(logits) and score_function in SCORE_FUNCTIONS:
-        out = _native.ext.topk_router(logits, expert_bias, topk, SCORE_FUNCTIONS[score_function], num_groups, topk_groups, normalize, scaling_factor, dense)
+    if _native.usable(logits) and type(topk) is type(num_groups) is type(topk_groups) is int and score_function in SCORE_FUNCTIONS:
+        out = _native.ext.topk_router(logits, expert_bias, topk, SCORE_FUNCTIONS[score_function], num_groups, topk_groups, bool(normalize),
+                                      float(scaling_factor), dense)
         if out is not None:
             return out
     if logits.dim() != 2:

@@ -215,3 +215,35 @@ def test_offsets_past_32_bits():
     assert v[-1, 2] == 1.0 and v[-1].sum() == 1.0
     again = quantize_int4(v, 128)
     assert torch.equal(again.codes()[-1, :4].cpu(), torch.tensor([8, 8, 15, 8], dtype=torch.uint8)) and bool((again.qdata[:-1] == q.qdata).all())
+
+
+@pytest.mark.parametrize("m", [13, 24, 64])
+def test_a_batch_is_repeatable_and_captured(m):
+    """Rows of x that share k among the CTAs of a cluster."""
+    q = weight((520, 6152), 32, True)
+    x = torch.randn(m, 6152, device=DEV, dtype=torch.float16)
+    y = gemm_int4(x, q)
+    assert_product(y, x, q)
+    assert all(torch.equal(y, gemm_int4(x, q)) for _ in range(5))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        z = gemm_int4(x, q)
+    x.copy_(torch.randn_like(x))
+    graph.replay()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        y = gemm_int4(x, q)
+        torch.cuda.synchronize()
+    assert torch.equal(z, y)
+
+
+def test_scales_that_start_anywhere():
+    """Groups whose scales and zero points lie at odd places of their memory."""
+    for group in (32, 64):
+        q = weight((64, 1024), group, True)
+        x = torch.randn(20, 1024, device=DEV, dtype=torch.bfloat16)
+        s, z = torch.empty(q.scale.numel() + 1, device=DEV, dtype=torch.bfloat16), torch.empty(q.zero.numel() + 1, device=DEV, dtype=torch.uint8)
+        s[1:].copy_(q.scale.flatten())
+        z[1:].copy_(q.zero.flatten())
+        other = Int4Weight(q.qdata, s[1:].view(q.scale.shape), z[1:].view(q.zero.shape), q.shape, group)
+        for rows in (1, 20):
+            assert torch.equal(gemm_int4(x[:rows], other), gemm_int4(x[:rows], q))

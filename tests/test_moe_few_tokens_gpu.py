@@ -274,3 +274,37 @@ def test_the_same_layer_as_in_training():
     y = moe_few_tokens(x, ids, probs, w1, w2)
     off = (y.double() - want.double()).norm(dim=1) / want.double().norm(dim=1)
     assert bool((off < 2 * 2.0**-4).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_an_expert_with_most_of_the_tokens(fmt, dtype):
+    """Fewer columns a pass than an expert has tokens, where the others have few."""
+    w1, w2 = layer(8, 272, 144, fmt, dtype)
+    ids = torch.full((60, 1), 3, device=DEV)
+    ids[::7] = 5
+    assert_layer(torch.randn(60, 272, device=DEV).to(dtype), ids, torch.rand(60, 1, device=DEV) + 0.1, w1, w2)
+
+
+@pytest.mark.parametrize("fmt", ["raw", "block", "int4_32"])
+def test_batches_in_two_graphs_and_between_them(fmt):
+    w1, w2 = layer(6, 512, 256, fmt)
+    ids, probs = routed(40, 6, 2)
+    xs = [torch.randn(40, 512, device=DEV, dtype=torch.bfloat16) for _ in range(3)]
+    want = [moe_few_tokens(x, ids, probs, w1[0], w2[0]) for x in xs]
+    held, outs, graphs = [x.clone() for x in xs[:2]], [], []
+    for x in held:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(moe_few_tokens(x, ids, probs, w1[0], w2[0]))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(5):
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        with torch.cuda.stream(streams[2]):
+            y = moe_few_tokens(xs[2], ids, probs, w1[0], w2[0])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(y, want[2])

@@ -462,6 +462,7 @@ __device__ __forceinline__ void few_rows_walk(float (&acc)[NT][4], uint8_t *smem
     using W = Walk<FMT, NT, WR>;
     using Piece = RowPiece<FMT>;
     constexpr int CB = kChunk<FMT>;
+    static_assert(kTerms * NT <= WR && (WR & (WR - 1)) == 0, "the warps copy eight rows of x each");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int live = (cols + 7) / 8, x_rows = kTerms * cols, x_warps = (x_rows + 7) / 8;
     const uint32_t ring = shared_u32(smem) + warp * (kWeightSlots * kSlotBytes), x_ring = shared_u32(smem) + WR * (kWeightSlots * kSlotBytes), x_stage = x_rows * kXPitch;

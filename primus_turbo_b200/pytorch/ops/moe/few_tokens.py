@@ -55,7 +55,7 @@ def _parts(name: str, w: Weight, dtype: torch.dtype):
 def _native_layer(x, ids, probs, w1, w2):
     """The call through the native host path; ``None`` where it has to run in Python."""
     if type(w1) is Int4Weight and type(w2) is Int4Weight:
-        if len(w1.shape) != 3 or len(w2.shape) != 3 or w1.group_size != w2.group_size or w1.shape[2] != x.shape[-1]:
+        if x.dim() != 2 or len(w1.shape) != 3 or len(w2.shape) != 3 or w1.group_size != w2.group_size or w1.shape[2] != x.shape[-1]:
             return None
         return _native.ext.moe_few_tokens(x, ids, probs, w1.qdata, w1.scale, w1.zero, w2.qdata, w2.scale, w2.zero, w2.shape[2], 0, w1.group_size)
     if isinstance(w1, QuantizedTensor) and isinstance(w2, QuantizedTensor):

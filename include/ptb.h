@@ -463,7 +463,7 @@ int ptb_topk_router_bwd(const void *logits, int dtype, int64_t T, int64_t E, int
 /* ------------------------------------------------------------------ 4-bit weights ------------- */
 /* A 4-bit weight of rows x K values: codes, ceil(K / 128) * 64 bytes a row, and per group of 32, 64 or 128 neighbouring values
  * of a row a bf16 scale and (optionally) a zero point byte, both [rows, ceil(K / group)].  value = (code - zero) * scale; zero is
- * 8 where zero is NULL.  In a row's block of 128 values, the 32-bit word t * 4 + q (t, q in 0 .. 3) holds the eight values from 32 q +
+ * any byte, 8 where zero is NULL.  In a row's block of 128 values, the 32-bit word t * 4 + q (t, q in 0 .. 3) holds the eight values from 32 q +
  * 8 t on: value i of them in bits 8 (i % 4) + 4 (i / 4) on.  Codes past K are 0.  K a multiple of 8; codes 16-byte aligned.
  *
  * Quantise: w [rows, K] contiguous, 16-byte aligned, fp32 / fp16 / bf16.

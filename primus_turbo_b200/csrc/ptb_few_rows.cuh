@@ -44,7 +44,7 @@ template <int FMT> constexpr bool kScaledX = FMT != kW16; // x is scaled per blo
 
 // 4-bit weights.  Row n of a [N, K] weight is ceil(K / 128) blocks of 64 bytes.  Word t * 4 + q of a block holds octet (q, t), so lane t
 // of a quad reads its four octets as one 16-byte piece.  Byte i of a word holds code i of the eight in its low nibble and code
-// i + 4 in its high one.  Codes past K are 0.   value = (code - zero) * scale, zero = 8 where no zero points are given.
+// i + 4 in its high one.  Codes past K are 0.   value = (code - zero) * scale with any byte as zero, 8 where no zero points are given.
 constexpr int kInt4BlockBytes = 64;
 __device__ __forceinline__ int int4_shift(int i) { return (i & 3) * 8 + (i >> 2) * 4; } // of code i of a word
 
@@ -327,11 +327,10 @@ template <int FMT, int G> struct BlockScale {
         if constexpr (FMT != kWInt4) return __uint_as_float(s[0]);
         return __uint_as_float(i % 2 ? s[i / 2] & 0xffff0000u : s[i / 2] << 16);
     }
-    // -(1024 + zero) and -(64 + zero) in both halves: fp16 numbers whose last bit is worth 1 or 1 / 16
+    // -(1024 + zero) and -(64 + zero) in both halves, exact for every byte: fp16 numbers whose last bit is worth 1
     __device__ __forceinline__ void minus_zero(int i, uint32_t &za, uint32_t &zb) const {
-        const uint32_t both = __byte_perm(z, 0, 0x4040 | i | i << 8);
-        za = both + 0xe400e400u;
-        zb = both * 16 + 0xd400d400u;
+        za = __byte_perm(z, 0, 0x4040 | i | i << 8) + 0xe400e400u;
+        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(zb) : "r"(za), "r"(0x63806380u)); // plus 960
     }
 };
 

@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(256) int4_dequant_kernel(const uint4 *codes, c
         const int64_t at = (int64_t) row * groups + ((k0 + 32 * q) >> log_group);
         const uint32_t z = zero != nullptr ? zero[at] : 8;
         uint4 *to        = reinterpret_cast<uint4 *>(out + (int64_t) row * K + k);
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        if (std::is_same<T, __nv_bfloat16>::value && z < 128) { // 128 + zero is a bf16 up to there
             const __nv_bfloat16 s = scale[at];
             const __nv_bfloat162 s2{s, s};
             const uint32_t base = 0x43004300u + z * 0x00010001u; // 128 + zero

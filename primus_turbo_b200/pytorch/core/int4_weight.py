@@ -1,6 +1,6 @@
 """``Int4Weight``: a weight of 4-bit codes with a scale (and optionally a zero point) per group of a row.
 
-``value[..., n, k] = (code - zero) * scale`` with one bf16 ``scale`` and one byte ``zero`` (8 where there are none) per
+``value[..., n, k] = (code - zero) * scale`` with one bf16 ``scale`` and one byte ``zero`` (any; 8 where there are none) per
 ``group_size`` neighbouring ``k`` of a row.  ``qdata`` holds the codes as the kernels read them, ``ceil(K / 128) * 64`` bytes a
 row (the order is described in ``include/ptb.h``); ``from_codes`` and ``codes`` convert from and to one code a byte.
 """

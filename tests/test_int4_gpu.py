@@ -247,3 +247,24 @@ def test_scales_that_start_anywhere():
         other = Int4Weight(q.qdata, s[1:].view(q.scale.shape), z[1:].view(q.zero.shape), q.shape, group)
         for rows in (1, 20):
             assert torch.equal(gemm_int4(x[:rows], other), gemm_int4(x[:rows], q))
+
+
+@pytest.mark.parametrize("m", [1, 8, 9, 40])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_zero_points_of_any_byte(m, group, dtype):
+    q = weight((72, 520), group, True)
+    zero = (torch.arange(q.zero.numel(), device=DEV) * 37 % 256).to(torch.uint8).view(q.zero.shape)
+    q = Int4Weight(q.qdata, q.scale, zero, q.shape, group)
+    w = values(q)
+    for t in (torch.bfloat16, torch.float16, torch.float32):
+        v = dequantize_int4(q, t).double()
+        assert bool(((v - w).abs() <= w.abs() * torch.finfo(t).eps / 2).all())  # values below 2^-14 do not occur: scales are 2^-6 and more
+    x = torch.randn(m, 520, device=DEV).to(dtype)
+    xd, s = x.double(), spread(q.scale, group, 520).double()
+    want = xd @ w.T
+    # as in assert_product, with zero points up to 255 in the place of 15: sums of codes and zero times the sum of x, up to 270 steps together
+    size = (xd.abs() @ w.abs().T) * (520 / 1024 + 31) + xd.abs() @ s.T * (270 * 12)
+    tol = size * 2.0**-23 + xd.abs().amax(1, keepdim=True) * w.abs().sum(1) * 2.0**-15 + want.abs() * torch.finfo(dtype).eps / 2
+    y = gemm_int4(x, q).double()
+    assert bool(((y - want).abs() <= tol).all()), ((y - want).abs() / tol).max()

@@ -580,6 +580,34 @@ __device__ __forceinline__ void few_rows_walk(float (&acc)[NT][4], uint8_t *smem
     if (threadIdx.x < W::kBars) bar_end(shared_u32(bars) + threadIdx.x * 8);
 }
 
+// The CTAs of a cluster may share k, each a run of four blocks or more (whole chunks and pairs); each adds up a part of the results, in the order of k.
+constexpr int kShareBlocks = 4;
+struct Share {
+    int begin, end; // blocks
+};
+__device__ __forceinline__ Share share_of(int K, int share, int shares) {
+    const int blocks = (K + kKB - 1) / kKB, runs = (blocks + kShareBlocks - 1) / kShareBlocks;
+    return {share * runs / shares * kShareBlocks, min(blocks, (share + 1) * runs / shares * kShareBlocks)};
+}
+// As many as it takes to give every place of the device a CTA.  Without: 64 rows, 8192 x 8192 in 4 bits (128 CTAs, 256 with), 83 instead of 49 us;
+// an MoE layer of 16 tokens, 2 of 8 experts of 7168 x 256, 45 instead of 24 us.
+inline int shares_for(int K, int64_t ctas, int places) {
+    int shares = 1;
+    while (shares < 8 && 2 * shares <= cdiv(K, kKB * kShareBlocks) && ctas * shares * 2 <= places) shares *= 2;
+    return shares;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float read_peer(const float *p, uint32_t rank) {
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(shared_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+
 // The sums in shared memory [column][row].
 template <int FMT, int NT, int WR> struct RowSums {
     static constexpr int kPitch = Walk<FMT, NT, WR>::kRows + 1;
@@ -592,7 +620,12 @@ template <int FMT, int NT, int WR> struct RowSums {
             for (int j = 0; j < 4; ++j) part[(i * 8 + 2 * t + (j & 1)) * kPitch + warp * 16 + lane_row() + (j >> 1) * 8] = acc[i][j];
         __syncthreads();
     }
-    __device__ __forceinline__ float sum(int column, int row) const { return part[column * kPitch + row]; }
+    __device__ __forceinline__ float sum(int column, int row, int shares) const { // shares > 1: between two cluster_sync
+        float *at = &part[column * kPitch + row], s = 0.0f;
+        if (shares == 1) return *at;
+        for (int r = 0; r < shares; ++r) s += read_peer(at, r);
+        return s;
+    }
 };
 
 // ---- scaling rows of x -------------------------------------------------------------------------------------------------------

@@ -273,17 +273,6 @@ template <int G> struct Int4BatchRows : Int4Rows<G> {
     int row0;
     __device__ __forceinline__ const uint8_t *x(int, int col) const { return xs.planes + (row0 + col) * xs.pitch; }
 };
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float read_peer(const float *p, uint32_t rank) {
-    uint32_t at;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(shared_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-    return v;
-}
 template <typename T, int G, int NT, int WR>
 __global__ void __launch_bounds__(32 * WR, 16 / WR) int4_gemm_kernel(const __grid_constant__ Int4GemmArgs a, int shares, int per) {
     extern __shared__ __align__(16) uint8_t raw[];
@@ -292,22 +281,19 @@ __global__ void __launch_bounds__(32 * WR, 16 / WR) int4_gemm_kernel(const __gri
     __shared__ uint64_t bars[W::kBars];
     const int tile = blockIdx.x / shares, share = blockIdx.x % shares; // (the rank in the cluster)
     const int n0 = tile * W::kRows, m0 = blockIdx.y * per, cols = min(per, a.M - m0);
-    const int blocks = (a.K + kKB - 1) / kKB, chunks = (blocks + kChunk<kWInt4> - 1) / kChunk<kWInt4>;
+    const Share k = share_of(a.K, share, shares);
     Int4BatchRows<G> src;
     src.aim(a, n0 + (threadIdx.x >> 5) * 16);
     src.xs   = a.xs;
     src.row0 = m0;
     float acc[NT][4] = {};
-    few_rows_walk<T, kWInt4, G, 128, NT, WR, 1, false>(acc, smem, bars, &a.map, a.K, cols, share * chunks / shares * kChunk<kWInt4>,
-                                                       min(blocks, (share + 1) * chunks / shares * kChunk<kWInt4>), src);
+    few_rows_walk<T, kWInt4, G, 128, NT, WR, 1, false>(acc, smem, bars, &a.map, a.K, cols, k.begin, k.end, src);
     const RowSums<kWInt4, NT, WR> sums(acc, smem);
     if (shares > 1) cluster_sync();
     for (int i = threadIdx.x + share * W::kThreads; i < cols * W::kRows; i += W::kThreads * shares) {
         const int m = i / W::kRows, n = i % W::kRows;
         if (n0 + n >= a.N) continue;
-        float s = 0.0f;
-        if (shares == 1) s = sums.sum(m, n);
-        else for (int r = 0; r < shares; ++r) s += read_peer(&sums.part[m * sums.kPitch + n], r);
+        float s = sums.sum(m, n, shares);
         if (a.bias != nullptr) s += to_f32(((const T *) a.bias)[n0 + n]);
         ((T *) a.out)[(int64_t) (m0 + m) * a.N + n0 + n] = from_f32<T>(s);
     }
@@ -319,9 +305,8 @@ template <typename T, int G, int NT, int WR> int launch_tile(const Int4GemmArgs 
     int sms = 0;
     if (int rc = sm_count(&sms)) return rc;
     const int per = cdiv(cdiv(a.M, cdiv(a.M, NT * 8)), 8) * 8, sets = cdiv(a.M, per); // rows of x a CTA, eights as even as can be
-    const int tiles = cdiv(a.N, W::kRows), chunks = cdiv(a.K, kKB * kChunk<kWInt4>);
-    int shares = 1; // of k: as many as it takes to give every SM its 16 warps
-    while (shares < 8 && 2 * shares <= chunks && (int64_t) tiles * sets * shares * 2 <= (int64_t) sms * (16 / WR)) shares *= 2;
+    const int tiles = cdiv(a.N, W::kRows);
+    const int shares = shares_for(a.K, (int64_t) tiles * sets, sms * (16 / WR));
     PTB_CUDA(launch_early(int4_gemm_kernel<T, G, NT, WR>, dim3((unsigned) (tiles * shares), (unsigned) sets), W::kThreads,
                           (size_t) W::smem(1, (int) imin(a.M, per)), st, (unsigned) shares, a, shares, per));
     PTB_LAUNCH_CHECK("int4_gemm_kernel");

@@ -308,3 +308,15 @@ def test_batches_in_two_graphs_and_between_them(fmt):
             y = moe_few_tokens(xs[2], ids, probs, w1[0], w2[0])
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(y, want[2])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("T,E,k,H,I", [(9, 2, 1, 1168, 656), (12, 4, 2, 2000, 1040), (40, 2, 2, 4112, 528)])
+def test_few_experts_share_k(fmt, T, E, k, H, I):
+    """So few experts that the CTAs of a cluster share k, in parts that end inside a run of blocks."""
+    dtype = torch.float16 if T == 12 else torch.bfloat16
+    w1, w2 = layer(E, H, I, fmt, dtype, seed=T)
+    ids, probs = routed(T, E, k, seed=T)
+    x = torch.randn(T, H, device=DEV).to(dtype)
+    y = assert_layer(x, ids, probs, w1, w2)
+    assert torch.equal(y, moe_few_tokens(x, ids, probs, w1[0], w2[0]))

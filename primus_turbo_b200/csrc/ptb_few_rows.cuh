@@ -15,7 +15,7 @@
 //     and an unsigned low one.  bf16's eight bits are exact in it down to 2^-7 of the largest; below, a value is off by up to 2^-15 of
 //     the largest.  Sums of a group are exact integers, and scaling them is what costs: with more columns of x than eight it is too much;
 //   * for more (few_rows_walk) codes become fp16 less their zero, exactly, 9 instructions for 8.  That is what bounds it: 48 tokens through 32
-//     experts of 7168 x 2048, groups of 32, 357 us where the weights' 790 MB are 121, with two thirds of all issue slots used.  Of these, scaling
+//     experts of 7168 x 2048, groups of 32, 351 us where the weights' 790 MB are 121, with two thirds of all issue slots used.  Of these, scaling
 //     the sums of the groups and their MMAs are a fifth, unpacking an eighth, fetching scales a tenth;
 //   * FP8 weights are converted to fp16, exactly, one instruction for two;
 //   * x goes with fp16 weights as fp16, scaled by a power of two per block into its range, where bf16 and fp16 values are exact down

@@ -289,5 +289,5 @@ for _name in ("quantize_fp8_tensorwise", "quantize_fp8_rowwise", "quant_fp8_bloc
               "quant_fp8_blockwise_for_weight", "quant_fp8_blockwise_segment_m_row_col", "dequantize_fp8", "gemm_fp8_impl",
               "grouped_gemm_fp8_impl", "grouped_gemm_fp8_variable_k_impl", "topk_router", "topk_router_bwd", "quant_int4",
               "dequant_int4", "gemm_int4", "moe_few_tokens"):
-    globals()[_name] = _with_eager_fast_path(globals()[_name], _name in ("gemm_int4", "moe_few_tokens"))
+    globals()[_name] = _with_eager_fast_path(globals()[_name], _name in ("quant_int4", "dequant_int4", "gemm_int4", "moe_few_tokens"))
 del _name

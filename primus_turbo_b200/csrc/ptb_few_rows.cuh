@@ -55,17 +55,20 @@ __device__ __forceinline__ int int4_shift(int i) { return (i & 3) * 8 + (i >> 2)
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dep_open() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// Shared memory: `smem` for this launch, `most` for any.  The limit that is set belongs to the kernel, not to the launch, and another thread may launch
+// the same kernel with other sizes between the two calls here: so it is the same number every time.
 template <typename... P, typename... A>
-inline cudaError_t launch_early(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, unsigned cluster, A &&...args) {
+inline cudaError_t launch_early(void (*kernel)(P...), dim3 grid, unsigned threads, int smem, int most, cudaStream_t st, unsigned cluster, A &&...args) {
+    if (smem > most) return cudaErrorInvalidValue;
     if (smem > 32 * 1024) // 48 KB without asking, with what the kernel has besides
-        if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem)) return e;
+        if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most)) return e;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[2] = {};
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim = {cluster, 1, 1};
-    cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = (size_t) smem; cfg.stream = st;
     cfg.attrs = attr; cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
@@ -426,7 +429,7 @@ template <int FMT, int NT, int WR> struct Walk {
     static constexpr int kBars = WR * kWeightSlots + 2 * kPair;
     static constexpr int kSums = NT * 8 * (kRows + 1) * 4;
     // what the CTA's shared memory has to hold: the slots and the ring, read to the end of eight columns, then the sums and `more`
-    static int smem(int terms, int cols, int more = 0) {
+    static constexpr int smem(int terms, int cols, int more = 0) {
         const int a = WR * kWeightSlots * kSlotBytes + (2 * terms * cols + 7) * kXPitch, b = kSums + more;
         return (a > b ? a : b) + kAlign;
     }

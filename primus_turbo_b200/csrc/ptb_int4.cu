@@ -307,8 +307,9 @@ template <typename T, int G, int NT, int WR> int launch_tile(const Int4GemmArgs 
     const int per = cdiv(cdiv(a.M, cdiv(a.M, NT * 8)), 8) * 8, sets = cdiv(a.M, per); // rows of x a CTA, eights as even as can be
     const int tiles = cdiv(a.N, W::kRows);
     const int shares = shares_for(a.K, (int64_t) tiles * sets, sms * (16 / WR));
+    constexpr int kMost = W::smem(1, NT * 8);
     PTB_CUDA(launch_early(int4_gemm_kernel<T, G, NT, WR>, dim3((unsigned) (tiles * shares), (unsigned) sets), W::kThreads,
-                          (size_t) W::smem(1, (int) imin(a.M, per)), st, (unsigned) shares, a, shares, per));
+                          W::smem(1, (int) imin(a.M, per)), kMost, st, (unsigned) shares, a, shares, per));
     PTB_LAUNCH_CHECK("int4_gemm_kernel");
     return 0;
 }
@@ -321,12 +322,12 @@ template <typename T, int G> int launch_gemm(const Int4GemmArgs &a, cudaStream_t
         int sms = 0;
         if (int rc = sm_count(&sms)) return rc;
         const int tiles = cdiv(a.N, 16), shares = token_shares(tiles, cdiv(a.K, kKB), sms);
-        PTB_CUDA(launch_early(int4_token_kernel<T, G>, dim3((unsigned) cdiv(tiles, kTokenWarps >> shares)), 32 * kTokenWarps, (size_t) token_smem(x_bytes, a.M), st, 1, a, shares));
+        PTB_CUDA(launch_early(int4_token_kernel<T, G>, dim3((unsigned) cdiv(tiles, kTokenWarps >> shares)), 32 * kTokenWarps, token_smem(x_bytes, a.M), kMostSmem, st, 1, a, shares));
         PTB_LAUNCH_CHECK("int4_token_kernel");
         return 0;
     }
     const int64_t warps = a.M * cdiv<int64_t>(a.K, kKB);
-    PTB_CUDA(launch_early(scale_rows_kernel<T, kWInt4>, dim3((unsigned) cdiv<int64_t>(warps, 4)), 128, 0, st, 1, (const T *) a.x, a.ldx, a.M, a.K, a.xs));
+    PTB_CUDA(launch_early(scale_rows_kernel<T, kWInt4>, dim3((unsigned) cdiv<int64_t>(warps, 4)), 128, 0, 0, st, 1, (const T *) a.x, a.ldx, a.M, a.K, a.xs));
     PTB_LAUNCH_CHECK("scale_rows_kernel");
     if (a.M <= 8) return launch_tile<T, G, 1, 4>(a, st);
     if (a.M <= 16) return launch_tile<T, G, 2, 4>(a, st);

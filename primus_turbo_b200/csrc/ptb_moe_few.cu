@@ -470,9 +470,9 @@ template <typename T, int FMT, int G> int launch_token(const LayerArgs &a, int u
     const int hits = (int) imin(a.E, a.T * a.k), up_tiles = hits * cdiv(a.I, 8), down_tiles = cdiv(a.H, 16);
     const int up_shares = token_shares(up_tiles, cdiv(a.H, kKB), sms), down_shares = token_shares(down_tiles, hits * cdiv(a.I, kKB), sms);
     const dim3 g1((unsigned) cdiv(up_tiles, kTokenWarps >> up_shares)), g2((unsigned) cdiv(down_tiles, kTokenWarps >> down_shares));
-    PTB_CUDA(launch_early(moe_gate_up_token_kernel<T, FMT, G>, g1, 32 * kTokenWarps, (size_t) up, st, 1, a, up_shares));
+    PTB_CUDA(launch_early(moe_gate_up_token_kernel<T, FMT, G>, g1, 32 * kTokenWarps, up, kMostSmem, st, 1, a, up_shares));
     PTB_LAUNCH_CHECK("moe_gate_up_token_kernel");
-    PTB_CUDA(launch_early(moe_down_token_kernel<T, FMT, G>, g2, 32 * kTokenWarps, (size_t) down, st, 1, a, down_shares));
+    PTB_CUDA(launch_early(moe_down_token_kernel<T, FMT, G>, g2, 32 * kTokenWarps, down, kMostSmem, st, 1, a, down_shares));
     PTB_LAUNCH_CHECK("moe_down_token_kernel");
     return 0;
 }
@@ -481,18 +481,19 @@ template <typename T, int FMT, int G, int NT> int launch_batch(const LayerArgs &
     using W = Walk<FMT, NT, kWarps>;
     const unsigned hits = (unsigned) imin(a.E, a.T * a.k), splits = kScaledX<FMT> ? (unsigned) cdiv(a.T * cdiv(a.H, kKB), 32) : 0u;
     const int cols = (int) imin(a.T, NT * 8);
-    const int up_smem = W::smem(1, cols, NT * 8 * (kChannels + 1) * 4), down_smem = W::smem(kDownTerms<T, FMT>, cols);
-    PTB_CUDA(launch_early(moe_list_kernel<T, FMT>, dim3(1 + splits), 1024, 0, st, 1, a.ids, a.probs, a.T, a.k, a.E, a.lists, (const T *) a.x, a.ldx, a.H, a.xs));
+    constexpr int kMore = NT * 8 * (kChannels + 1) * 4, kUpMost = W::smem(1, NT * 8, kMore), kDownMost = W::smem(kDownTerms<T, FMT>, NT * 8);
+    const int up_smem = W::smem(1, cols, kMore), down_smem = W::smem(kDownTerms<T, FMT>, cols);
+    PTB_CUDA(launch_early(moe_list_kernel<T, FMT>, dim3(1 + splits), 1024, 0, 0, st, 1, a.ids, a.probs, a.T, a.k, a.E, a.lists, (const T *) a.x, a.ldx, a.H, a.xs));
     PTB_LAUNCH_CHECK("moe_list_kernel");
     int sms = 0;
     if (int rc = sm_count(&sms)) return rc;
     const unsigned channels = (unsigned) (kScaledX<FMT> ? cdiv(a.I, kKB) * 2 : cdiv(a.I, kChannels)), rows = (unsigned) cdiv(a.H, W::kRows); // CTAs; h's planes are whole blocks
     const unsigned up = (unsigned) shares_for(a.H, (int64_t) channels * hits, 2 * sms), down = (unsigned) shares_for(a.I, (int64_t) rows * hits, 2 * sms);
-    PTB_CUDA(launch_early(up > 1 ? moe_gate_up_kernel<T, FMT, G, NT, true> : moe_gate_up_kernel<T, FMT, G, NT, false>, dim3(channels * up, hits), W::kThreads, (size_t) up_smem, st, up, a, (int) up));
+    PTB_CUDA(launch_early(up > 1 ? moe_gate_up_kernel<T, FMT, G, NT, true> : moe_gate_up_kernel<T, FMT, G, NT, false>, dim3(channels * up, hits), W::kThreads, up_smem, kUpMost, st, up, a, (int) up));
     PTB_LAUNCH_CHECK("moe_gate_up_kernel");
-    PTB_CUDA(launch_early(down > 1 ? moe_down_kernel<T, FMT, G, NT, true> : moe_down_kernel<T, FMT, G, NT, false>, dim3(rows * down, hits), W::kThreads, (size_t) down_smem, st, down, a, (int) down));
+    PTB_CUDA(launch_early(down > 1 ? moe_down_kernel<T, FMT, G, NT, true> : moe_down_kernel<T, FMT, G, NT, false>, dim3(rows * down, hits), W::kThreads, down_smem, kDownMost, st, down, a, (int) down));
     PTB_LAUNCH_CHECK("moe_down_kernel");
-    PTB_CUDA(launch_early(moe_merge_kernel<T>, dim3((unsigned) cdiv(a.H, 1024), (unsigned) a.T), 128, 0, st, 1, a));
+    PTB_CUDA(launch_early(moe_merge_kernel<T>, dim3((unsigned) cdiv(a.H, 1024), (unsigned) a.T), 128, 0, 0, st, 1, a));
     PTB_LAUNCH_CHECK("moe_merge_kernel");
     return 0;
 }

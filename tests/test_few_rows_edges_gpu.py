@@ -8,7 +8,7 @@ import torch
 
 from primus_turbo_b200 import _lib
 from primus_turbo_b200.pytorch.core.int4_weight import Int4Weight
-from primus_turbo_b200.pytorch.ops import gemm_int4
+from primus_turbo_b200.pytorch.ops import dequantize_int4, gemm_int4, quantize_int4
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -55,3 +55,10 @@ def test_two_threads_launch_one_kernel_with_different_sizes():
     torch.cuda.synchronize()
     assert failed == [0, 0]
     assert all(torch.equal(a, b) for o, w in zip(out, want) for a, b in zip(o, w))
+
+
+def test_traced_quantising_runs_again_on_new_inputs():
+    w, x, other = quantize_int4(torch.randn(72, 256, device=DEV, dtype=BF), 128), *(torch.randn(3, 256, device=DEV, dtype=BF) for _ in range(2))
+    for f in (lambda x: x @ dequantize_int4(w).T, lambda x: quantize_int4(x, 32).qdata, lambda x: dequantize_int4(quantize_int4(x, 32, False))):
+        traced = torch.jit.trace(f, (x,), check_trace=False)
+        assert torch.equal(traced(other), f(other)) and torch.equal(traced(x), f(x))

@@ -476,7 +476,8 @@ int ptb_quant_int4(const void *w, int dtype, int64_t rows, int64_t K, int64_t gr
 int ptb_dequant_int4(const void *codes, const void *scale, const void *zero, int64_t rows, int64_t K, int64_t group,
                      void *out, int out_dtype, ptb_stream_t stream);
 /* out[m, n] = sum_k x[m, k] * value[n, k] (+ bias[n]), accumulated in fp32; x [M, K] with rows ldx apart (a multiple of 8
- * where M > 1, 16-byte aligned), bias [N] and out [M, N] in x's type (bf16 or fp16).  Made for few rows; more are taken 32 at a time,
+ * where M > 1, 16-byte aligned), bias [N] and out [M, N] in x's type (bf16 or fp16).  x is held to 2^-22 of the largest finite value of its 128
+ * (blocks of k) or better; bf16 and fp16 values above 2^-11 of that are exact.  Made for few rows; more are taken 32 at a time,
  * each time with another read of the weight.  workspace: 16-byte aligned, of ptb_gemm_int4_workspace bytes; calls that may overlap need
  * one each.  A row of x that holds a NaN or an infinity gives NaN and infinities. */
 int64_t ptb_gemm_int4_workspace(int dtype, int64_t M, int64_t K, int64_t group);
@@ -487,8 +488,10 @@ int ptb_gemm_int4(const void *x, int dtype, int64_t ldx, int64_t M, int64_t N, i
 /* ------------------------------------------------------------------ MoE layer for a few tokens - */
 /* out[t] = sum_j probs[t, j] * W2[e] (silu(u[:I]) * u[I:]), u = W1[e] x[t], e = ids[t, j], for W1 [E, 2 I, H] (gate rows first)
  * and W2 [E, H, I].  x [T, H] bf16 or fp16, rows ldx apart; ids [T, k] int64 and probs [T, k] fp32, contiguous; an id outside
- * [0, E) contributes nothing.  out [T, H] in x's type, contiguous.  Sums are kept in fp32, the activation between the two products
- * in fp16 or 16-bit integers scaled per 64 or 128 channels, with 16-bit weights or fp16 results in two parts; equal inputs give equal bits.
+ * [0, E) contributes nothing.  out [T, H] in x's type, contiguous.  x goes with 16-bit weights as it is,
+ * otherwise held to 2^-22 of the largest finite value of its 128 channels or better.  Sums are kept in fp32, the activation between the two products
+ * in fp16 scaled per 64 or 128 channels, with 16-bit weights or fp16 results in two parts, or as integers to 2^-22 of the largest of its 128 (4-bit
+ * weights, few tokens); equal inputs give equal bits.
  * format: x's own type code, PTB_E4M3, PTB_E5M2 or PTB_INT4, the same for both weights.  Data contiguous, 16-byte aligned.
  *   FP8: scale holds fp32 inverse scales, by granularity: PTB_TENSORWISE one, PTB_ROWWISE [E, rows], PTB_BLOCKWISE
  *        [E, ceil(rows / 128), ceil(K / 128)].  H and I multiples of 16.

@@ -10,10 +10,12 @@
 // What an MMA is fed with.  Measured on a B200, an SM issues an m16n8k16 of 16-bit floats or an m16n8k32 of bytes every 2.1 clocks (FP8
 // ones are taken apart into these: 5.6), and integer and conversion instructions at 64 lanes a clock; HBM brings 23 bytes a clock
 // and SM.  Unpacking 4-bit codes to bf16 is 7 such instructions for 8 codes, FP8 to bf16 8 for 4 values: too near the budget or beyond it.  So
-//   * for a token or a few (few_tokens_walk) 4-bit codes go in as the bytes they are: two ANDs and a shift for 8 codes.  x is a 16-bit
-//     integer per value, scaled by a power of two per block that brings the largest of its 128 to 2^14 .. 2^15, as a signed high byte
-//     and an unsigned low one.  bf16's eight bits are exact in it down to 2^-7 of the largest; below, a value is off by up to 2^-15 of
-//     the largest.  Sums of a group are exact integers, and scaling them is what costs: with more columns of x than eight it is too much;
+//   * for a token or a few (few_tokens_walk) 4-bit codes go in as the bytes they are: two ANDs and a shift for 8 codes.  x is an integer
+//     of three bytes, the first signed, scaled by a power of two per block that brings the largest of its 128 to 2^21 .. 2^22.  bf16's eight bits are
+//     exact in it down to 2^-14 of the largest, fp16's eleven to 2^-11; below, a value is off by up to 2^-22 of the largest.  (With two bytes 2^-15: beside
+//     an outlier of 1000 the result of the others is off by more than bf16's own rounding.  The third costs 5 %: 4096 x 14336, one row, 11.3 instead of
+//     10.7 us, and room: rows that no longer fit are for the other walk, 2 rows of 14336 19.5 instead of 13.5.)  Sums of
+//     a group are exact integers, and scaling them is what costs: with more columns of x than eight it is too much;
 //   * for more (few_rows_walk) codes become fp16 less their zero, exactly, 9 instructions for 8.  That is what bounds it: 48 tokens through 32
 //     experts of 7168 x 2048, groups of 32, 351 us where the weights' 790 MB are 121, with two thirds of all issue slots used.  Of these, scaling
 //     the sums of the groups and their MMAs are a fifth, unpacking an eighth, fetching scales a tenth;
@@ -187,7 +189,7 @@ __device__ __forceinline__ void block_scale(float largest, int top, float &scale
     scale = __uint_as_float((uint32_t) (e - top) << 23);
     inv   = __uint_as_float((uint32_t) (254 + top - e) << 23);
 }
-constexpr int kTopInt = 14, kTopHalf = 13;
+constexpr int kTopInt = 21, kTopHalf = 13;
 // Where value k of a block stands: among the bytes that go with byte codes (lane t's four octets are 32 neighbouring bytes), and among the
 // fp16 of the walk over rows (octet q of the four lanes: 64 neighbouring bytes; with 4-bit weights an octet's order is 0 2 1 3 4 6 5 7).
 __host__ __device__ __forceinline__ int byte_place(int k) { return (k / 8 % 4) * 32 + (k / 32) * 8 + k % 8; }

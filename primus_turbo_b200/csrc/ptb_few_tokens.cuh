@@ -21,6 +21,7 @@ namespace ptb {
 namespace {
 
 constexpr int kTokenWarps = 16, kTokenCols = 8;
+constexpr int kIntTerms = 3; // bytes of x beside 4-bit weights
 
 // x in shared memory: per block kTerms x cols rows (and once more, zeros), then per block and column the scales (and sums).
 template <int FMT, int G> struct TokenX {
@@ -72,27 +73,33 @@ __device__ __forceinline__ void stage_sixteen(uint8_t *x, uint8_t *runs, int blo
     if constexpr (FMT == kWInt4) {
         const unsigned bad = __ballot_sync(0xffffffffu, !fine);
         if (bad >> (lane & 24) & 255) scale = NAN; // integers hold no NaN and no infinity: the block's products become NaN
-        int n = 0;
+        uint32_t n = 0;
 #pragma unroll
         for (int o = 0; o < 2; ++o) {
-            uint32_t high[2] = {0, 0}, low[2] = {0, 0};
+            uint32_t high[2], mid[2], low[2];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                // rounded to an integer in the low bits of a float's mantissa
-                const int i = (int) (short) __float_as_int(fminf(v[o * 8 + j] * inv, 32767.0f) + kFloatBaseValue);
-                n += i;
-                high[j / 4] |= (uint32_t) (i >> 8 & 255) << (8 * (j % 4));
-                low[j / 4] |= (uint32_t) (i & 255) << (8 * (j % 4));
+            for (int j = 0; j < 2; ++j) {
+                uint32_t i[4];
+#pragma unroll
+                for (int l = 0; l < 4; ++l) { // rounded to an integer in the low bits of a float's mantissa
+                    i[l] = __float_as_uint(v[o * 8 + j * 4 + l] * inv + kFloatBaseValue) - (uint32_t) kFloatBase;
+                    n += i[l];
+                }
+                const uint32_t a = __byte_perm(i[0], i[1], 0x5140), b = __byte_perm(i[2], i[3], 0x5140);
+                low[j]  = __byte_perm(a, b, 0x5410);
+                mid[j]  = __byte_perm(a, b, 0x7632);
+                high[j] = __byte_perm(__byte_perm(i[0], i[1], 0x0062), __byte_perm(i[2], i[3], 0x0062), 0x5410);
             }
             const int at = byte_place(part * 16 + o * 8);
             if (here) {
-                *reinterpret_cast<uint2 *>(to + at)             = make_uint2(high[0], high[1]);
-                *reinterpret_cast<uint2 *>(to + next_term + at) = make_uint2(low[0], low[1]);
+                *reinterpret_cast<uint2 *>(to + at)                 = make_uint2(high[0], high[1]);
+                *reinterpret_cast<uint2 *>(to + next_term + at)     = make_uint2(mid[0], mid[1]);
+                *reinterpret_cast<uint2 *>(to + 2 * next_term + at) = make_uint2(low[0], low[1]);
             }
         }
 #pragma unroll
         for (int o = 1; o < G / 16; o <<= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-        if (here && part % (G / 16) == 0) reinterpret_cast<float2 *>(runs)[(block * cols + col) * X::kRuns + part / (G / 16)] = make_float2(scale, (float) n);
+        if (here && part % (G / 16) == 0) reinterpret_cast<float2 *>(runs)[(block * cols + col) * X::kRuns + part / (G / 16)] = make_float2(scale, (float) (int) n);
     } else {
         using H = std::conditional_t<FMT == kW16, T, __half>;
 #pragma unroll
@@ -193,7 +200,8 @@ __device__ __forceinline__ void few_tokens_walk(uint8_t *smem, const CUtensorMap
     }
     const uint32_t w_lane = ring + lane_place();
     using Sum = std::conditional_t<FMT == kWInt4, int, float>;
-    Sum c[2][4]; // 4-bit: products with high and with low bytes; otherwise two chains of MMAs, each waiting for its last
+    constexpr int kSums = FMT == kWInt4 ? kIntTerms : 2;
+    Sum c[kSums][4]; // 4-bit: products with high, middle and low bytes; otherwise two chains of MMAs, each waiting for its last
     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     uint32_t ws[2][2], wz[2][2]; // of the window: scale and zero point [column][row]
     Src here = src;
@@ -211,8 +219,8 @@ __device__ __forceinline__ void few_tokens_walk(uint8_t *smem, const CUtensorMap
             fresh = false;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                c[0][j] = FMT == kWInt4 ? (Sum) kFloatBase : (Sum) 0;
-                c[1][j] = c[0][j];
+#pragma unroll
+                for (int i = 0; i < kSums; ++i) c[i][j] = FMT == kWInt4 ? (Sum) kFloatBase : (Sum) 0;
             }
             if constexpr (FMT != kW16) {
                 const int groups = FMT == kWInt4 ? here.scale[0].count : blocks;
@@ -244,29 +252,31 @@ __device__ __forceinline__ void few_tokens_walk(uint8_t *smem, const CUtensorMap
                 Piece p[2];
                 p[0].read(from, i, 0);
                 p[1].read(from, i, 8 * 128);
-                uint4 u[2];
+                uint4 u[kIntTerms];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     if (q % kRun == 0 || q % 2 == 0) {
                         const uint32_t x = (filled + q / kRun == my_place ? x_here : zeros) + q / 2 * 16;
-                        u[0] = read16(x);
-                        u[1] = read16(x + term1);
+#pragma unroll
+                        for (int term = 0; term < kIntTerms; ++term) u[term] = read16(x + term * term1);
                     }
                     uint32_t lo[2], hi[2];
                     p[0].bytes(q, lo[0], hi[0]);
                     p[1].bytes(q, lo[1], hi[1]);
                     mma_8<true>(c[0], lo[0], lo[1], hi[0], hi[1], q % 2 ? u[0].z : u[0].x, q % 2 ? u[0].w : u[0].y);
                     mma_8<false>(c[1], lo[0], lo[1], hi[0], hi[1], q % 2 ? u[1].z : u[1].x, q % 2 ? u[1].w : u[1].y);
+                    mma_8<false>(c[kSums - 1], lo[0], lo[1], hi[0], hi[1], q % 2 ? u[2].z : u[2].x, q % 2 ? u[2].w : u[2].y);
                 }
             } else { // a window of one or two octets
                 const uint32_t w = (from + (i >> 1) * kBoxBytes) ^ (i & 1) * 64;
 #pragma unroll 1
                 for (int q = q0; q < q0 + unit; ++q) {
                     const uint32_t x = (filled + (q - q0) / kRun == my_place ? x_here : zeros) + q * 8;
-                    const uint2 u[2] = {read8u(x), read8u(x + term1)};
+                    const uint2 u[kIntTerms] = {read8u(x), read8u(x + term1), read8u(x + 2 * term1)};
                     const uint32_t wa = read4u(w + q * 4), wb = read4u(w + q * 4 + 8 * 128);
                     mma_8<true>(c[0], wa & 0x0f0f0f0fu, wb & 0x0f0f0f0fu, wa >> 4 & 0x0f0f0f0fu, wb >> 4 & 0x0f0f0f0fu, u[0].x, u[0].y);
                     mma_8<false>(c[1], wa & 0x0f0f0f0fu, wb & 0x0f0f0f0fu, wa >> 4 & 0x0f0f0f0fu, wb >> 4 & 0x0f0f0f0fu, u[1].x, u[1].y);
+                    mma_8<false>(c[kSums - 1], wa & 0x0f0f0f0fu, wb & 0x0f0f0f0fu, wa >> 4 & 0x0f0f0f0fu, wb >> 4 & 0x0f0f0f0fu, u[2].x, u[2].y);
                 }
             }
             filled += unit / kRun;
@@ -339,8 +349,10 @@ __device__ __forceinline__ void few_tokens_walk(uint8_t *smem, const CUtensorMap
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         if constexpr (FMT == kWInt4) {
-                            const float high = __int_as_float(c[0][2 * h + j]) - kFloatBaseValue, low = __int_as_float(c[1][2 * h + j]) - kFloatBaseValue;
-                            acc[2 * h + j] += (high * 256.0f + low - (float) wz[j][h] * xs.y) * (__uint_as_float(ws[j][h] << 16) * xs.x);
+                            const float high = __int_as_float(c[0][2 * h + j]) - kFloatBaseValue, mid = __int_as_float(c[1][2 * h + j]) - kFloatBaseValue,
+                                        low = __int_as_float(c[kSums - 1][2 * h + j]) - kFloatBaseValue;
+                            const float bare = __fmaf_rn(high, 65536.0f, __fmaf_rn(mid, 256.0f, low));
+                            acc[2 * h + j] += __fmaf_rn(-(float) wz[j][h], xs.y, bare) * (__uint_as_float(ws[j][h] << 16) * xs.x);
                         } else {
                             acc[2 * h + j] += (c[0][2 * h + j] + c[1][2 * h + j]) * (__uint_as_float(ws[j][h]) * xs.x);
                         }

@@ -245,10 +245,10 @@ template <typename T, int G> __global__ void __launch_bounds__(32 * kTokenWarps,
     extern __shared__ __align__(16) uint8_t raw[];
     uint8_t *smem = aligned(raw);
     const int lane = threadIdx.x & 31, blocks = (a.K + kKB - 1) / kKB;
-    few_tokens_walk<T, kWInt4, G, 2, false, false, false>(
+    few_tokens_walk<T, kWInt4, G, kIntTerms, false, false, false>(
         smem, &a.map, a.M, (a.N + 15) / 16, shares, 1, a.K, Int4TokenRows<G>(a),
         [&](uint8_t *x, uint8_t *runs) {
-            stage_blocks<T, T, kWInt4, G, 2>(x, runs, blocks, a.M, [&](int block, int col, int &left) {
+            stage_blocks<T, T, kWInt4, G, kIntTerms>(x, runs, blocks, a.M, [&](int block, int col, int &left) {
                 left = a.K - block * kKB;
                 return (const T *) a.x + col * a.ldx + block * kKB;
             });
@@ -317,7 +317,7 @@ template <typename T, int G, int NT, int WR> int launch_tile(const Int4GemmArgs 
 constexpr int kMostSmem = 227 * 1024 - 1024; // of a CTA, less what is not dynamic
 
 template <typename T, int G> int launch_gemm(const Int4GemmArgs &a, cudaStream_t st) {
-    const int x_bytes = a.M <= kTokenCols && a.K <= 1 << 20 ? TokenX<kWInt4, G>::bytes(2, a.M, cdiv(a.K, kKB)) : kMostSmem;
+    const int x_bytes = a.M <= kTokenCols && a.K <= 1 << 20 ? TokenX<kWInt4, G>::bytes(kIntTerms, a.M, cdiv(a.K, kKB)) : kMostSmem;
     if (token_smem(x_bytes, a.M) <= kMostSmem) {
         int sms = 0;
         if (int rc = sm_count(&sms)) return rc;

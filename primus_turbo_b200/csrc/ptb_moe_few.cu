@@ -19,8 +19,8 @@
 // experts of 2880 x 1440, 122 us where the weights are 61: its 368 CTAs have 296 places, and the second wave leaves three quarters of them empty.
 //
 // The activation h between the two products is kept in 32 bits and then scaled like x, or scaled at once, per 64 channels: to fp16
-// (2^-12 of each value; with fp16 results what that leaves is a second term), for 4-bit weights and few tokens to 16-bit integers.  With
-// 16-bit weights it is two bf16 (2^-17).  Its rounding is not felt in the result.
+// (2^-12 of each value; with fp16 results what that leaves is a second term), for 4-bit weights and few tokens to integers (2^-22 of the
+// block's largest).  With 16-bit weights it is two bf16 (2^-17).  Its rounding is not felt in the result.
 #include "ptb_few_tokens.cuh"
 
 namespace ptb {
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(32 * kTokenWarps, 1) moe_gate_up_token_kernel(
     __shared__ Pairs pairs;
     grid_dep_wait(); // the kernel before this one is somebody else's
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tiles = (a.I + 7) / 8, blocks = (a.H + kKB - 1) / kKB;
-    constexpr int kTerms = FMT == kWInt4 ? 2 : 1;
+    constexpr int kTerms = FMT == kWInt4 ? kIntTerms : 1;
     if (warp == 0) find_pairs(a, pairs);
     __syncthreads();
     few_tokens_walk<T, FMT, G, kTerms, false, false, false>(
@@ -279,7 +279,7 @@ template <int FMT> struct DownTokenRows : LaneRows<FMT> {
 };
 
 template <typename T> constexpr int kHScaled = std::is_same<T, __half>::value ? 2 : 1; // terms of scaled h
-template <typename T, int FMT> constexpr int kHTerms = FMT == kW16 || FMT == kWInt4 || std::is_same<T, __half>::value ? 2 : 1;
+template <typename T, int FMT> constexpr int kHTerms = FMT == kWInt4 ? kIntTerms : FMT == kW16 || std::is_same<T, __half>::value ? 2 : 1;
 
 template <typename T, int FMT, int G>
 __global__ void __launch_bounds__(32 * kTokenWarps, 1) moe_down_token_kernel(const __grid_constant__ LayerArgs a, int shares) {
@@ -459,7 +459,7 @@ constexpr int kMostSmem = 227 * 1024 - 4096; // of a CTA, less what is not dynam
 // Whether the two-kernel form has room for x and for h, and the shared memory of its kernels.
 template <typename T, int FMT, int G> bool fits_token(const LayerArgs &a, int &up, int &down) {
     if (a.T > kTokenCols || a.T * a.k > kTokenPairs || a.H > 1 << 17 || a.I > 1 << 15) return false;
-    up   = token_smem(TokenX<FMT, G>::bytes(FMT == kWInt4 ? 2 : 1, a.T, cdiv(a.H, kKB)), a.T);
+    up   = token_smem(TokenX<FMT, G>::bytes(FMT == kWInt4 ? kIntTerms : 1, a.T, cdiv(a.H, kKB)), a.T);
     down = token_smem(TokenX<FMT, G>::bytes(kHTerms<T, FMT>, a.T, (int) imin(a.E, a.T * a.k) * cdiv(a.I, kKB)), a.T);
     return up <= kMostSmem && down <= kMostSmem;
 }

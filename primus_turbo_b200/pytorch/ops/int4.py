@@ -74,7 +74,8 @@ def dequantize_int4(w: Int4Weight, out_dtype: torch.dtype = torch.bfloat16) -> t
 def gemm_int4(x: torch.Tensor, w: Int4Weight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ dequantised(w).T (+ bias)`` for ``x`` [..., K] (bf16 or fp16) and a 4-bit weight [N, K]; result [..., N] in x's type.
 
-    The activations stay in 16 bits and sums in fp32; the weight is never written out.  Made for few rows (a token, a decoding
+    Activations are held to 2^-22 of the largest of their 128 neighbours along K or better (what is above 2^-11 of it is exact), sums in
+    fp32; the weight is never written out.  Made for few rows (a token, a decoding
     batch): 32 rows are taken at a time, and beyond some hundreds ``dequantize_int4`` with a library product is the faster way.  A row
     of ``x`` that holds a NaN or an infinity gives NaN and infinities, other rows are not touched by it."""
     if not isinstance(w, Int4Weight):

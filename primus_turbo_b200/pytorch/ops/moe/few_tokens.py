@@ -80,8 +80,9 @@ def moe_few_tokens(
     with the gate rows first and ``w_down`` [E, H, I], both plain tensors of x's type, both FP8 ``QuantizedTensor`` (tensorwise, rowwise
     or 128 x 128 blockwise scales, of one kind), or both ``Int4Weight`` of one group size.  H and I are multiples of 8, of 16 for FP8.
 
-    Activations are not quantised.  Sums are kept in fp32, and the activation between the two products in more than bf16;
-    the result is rounded once to x's type.  Equal inputs give equal bits.  Every call allocates its own workspace, so calls on
+    Activations are not quantised: with FP8 and 4-bit weights they are held to 2^-22 of the largest of their 128 neighbours or better
+    (what is above 2^-11 of it is exact), with 16-bit weights as they are.  Sums are kept in fp32, and the activation between the two
+    products in more than bf16; the result is rounded once to x's type.  Equal inputs give equal bits.  Every call allocates its own workspace, so calls on
     several streams or in several captured graphs do not share any."""
     if _native.usable(x):
         y = _native_layer(x, topk_ids, topk_probs, w_gate_up, w_down)

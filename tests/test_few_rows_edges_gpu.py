@@ -9,10 +9,15 @@ import torch
 from primus_turbo_b200 import _lib
 from primus_turbo_b200.pytorch.core.int4_weight import Int4Weight
 from primus_turbo_b200.pytorch.ops import dequantize_int4, gemm_int4, quantize_int4
+from primus_turbo_b200.pytorch.ops.moe import moe_few_tokens
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 BF = torch.bfloat16
+
+
+def spread(t, group, k):
+    return t.repeat_interleave(group, dim=-1)[..., :k]
 
 
 def weight(shape, group, zeros, seed=0, codes=None):
@@ -22,6 +27,102 @@ def weight(shape, group, zeros, seed=0, codes=None):
     scale = ((torch.rand(groups, generator=g, device=DEV) + 0.5) * shape[-1] ** -0.5).to(BF)
     zero = torch.randint(0, 16, groups, generator=g, device=DEV, dtype=torch.uint8) if zeros else None
     return Int4Weight.from_codes(drawn if codes is None else codes, scale, zero, group_size=group)
+
+
+def parts(q):
+    """(values, scales, zero points) of every code, in 64 bits"""
+    k = q.shape[-1]
+    z = torch.full(q.shape, 8.0, device=DEV, dtype=torch.float64) if q.zero is None else spread(q.zero, q.group_size, k).double()
+    s = spread(q.scale, q.group_size, k).double()
+    return (q.codes().double() - z) * s, s, z
+
+
+def at_zero_point(q, channels):
+    """The weight with its codes of some channels at the zero point: what x holds there meets a value of zero."""
+    codes = q.codes()
+    codes[..., channels] = parts(q)[2][..., channels].to(torch.uint8)
+    return Int4Weight.from_codes(codes, q.scale, q.zero, group_size=q.group_size)
+
+
+# ---- outliers -----------------------------------------------------------------------------------------------------------------
+def product_bound(x, q, dtype):
+    """What a product of 4-bit weights may be off by.  x is held to 2^-22 of the largest of its 128 or better; bare codes, up to 15, are added up
+    exactly or in 32 bits, and zero (up to 15) times the sum of x is taken off: 12 operations of a group on sums of that size; then the
+    blocks of a warp (K / 1024 + 1), the warps and halves (20), each within 2^-23; one rounding to the output."""
+    w, s, _ = parts(q)
+    xd, k = x.double(), x.shape[-1]
+    want = xd @ w.T
+    ops = k / 1024 + 31
+    size = xd.abs() @ w.abs().T * ops + xd.abs() @ s.T * (30 * 12)
+    pad = lambda t: torch.nn.functional.pad(t, (0, -k % 128)).unflatten(-1, (-1, 128))  # noqa: E731
+    held = (pad(xd.abs()).amax(-1) @ pad(w.abs()).sum(-1).T) * 2.0**-22
+    return want, size * 2.0**-23 + held + want.abs() * torch.finfo(dtype).eps / 2
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 5, 8, 9, 16, 24])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype,outlier", [(torch.float16, 1000.0), (BF, 1000.0), (BF, 32768.0)])
+def test_small_activations_beside_an_outlier(m, group, zeros, dtype, outlier):
+    """A channel of 1000 among others of one, whose weights are zero: the result is that of the others, as exact as without it."""
+    k = 520
+    q = at_zero_point(weight((272, k), group, zeros, seed=group), [5, 130, 519])
+    x = torch.randn(m, k, device=DEV, generator=torch.Generator(DEV).manual_seed(m)).to(dtype)
+    x[:, [5, 130, 519]] = torch.tensor([outlier, -outlier, outlier / 3], device=DEV).to(dtype)
+    want, bound = product_bound(x, q, dtype)
+    y = gemm_int4(x, q).double()
+    assert bool(((y - want).abs() <= bound).all()), ((y - want).abs() / bound).max()
+
+
+def test_a_row_is_as_exact_in_a_small_batch_as_in_a_larger_one():
+    k = 2048
+    q = at_zero_point(weight((1024, k), 128, False), [77])
+    x = torch.randn(9, k, device=DEV, generator=torch.Generator(DEV).manual_seed(1)).to(torch.float16)
+    x[:, 77] = 3000.0
+    want = x.double() @ parts(q)[0].T
+    off = [((gemm_int4(x[:m], q).double() - want[:m]).norm() / want[:m].norm()).item() for m in (1, 8, 9)]
+    # rounding to fp16 leaves at most 2^-11 of each value; values held to 2^-22 of 3000 add at most 3000 x 2^-22 = 2^-10.4 of 1 to a sixteenth of the
+    # channels, a quarter of that in the norm, and fp32 sums beside it 12 x 30 / 4.6 x 2^-23 x 3000 / sqrt(2048) = 2^-10.7 at the very worst
+    assert all(o <= 2.0**-11 + 2.0**-12 + 2.0**-10 for o in off), off
+
+
+@pytest.mark.parametrize("T", [1, 2, 8, 9])
+@pytest.mark.parametrize("dtype", [BF, torch.float16])
+@pytest.mark.parametrize("where", ["x", "h"])
+def test_a_layer_beside_an_outlier(T, dtype, where):
+    """An outlier among the activations, or among what lies between the two products, at a channel whose weights are zero."""
+    E, H, I, k, group = 4, 384, 256, 2, 64
+    g = torch.Generator(DEV).manual_seed(T)
+    w1, w2 = weight((E, 2 * I, H), group, False, seed=1), weight((E, H, I), group, False, seed=2)
+    x = torch.randn(T, H, device=DEV, generator=g).to(dtype)
+    ids = torch.rand(T, E, device=DEV, generator=g).argsort(1)[:, :k].contiguous()
+    probs = torch.rand(T, k, device=DEV, generator=g) + 0.1
+    if where == "x":
+        w1, x[:, 9] = at_zero_point(w1, [9]), 1000.0
+    else:
+        scale = w1.scale.clone()
+        scale[:, I + 33] *= 1024  # of an up channel
+        w1, w2 = Int4Weight(w1.qdata, scale, None, w1.shape, group), at_zero_point(w2, [33])
+    (v1, s1, _), (v2, s2, _) = parts(w1), parts(w2)
+    y = moe_few_tokens(x, ids, probs, w1, w2).double()
+    eps = torch.finfo(dtype).eps / 2
+    blocks = lambda t: torch.nn.functional.pad(t, (0, -t.shape[-1] % 128)).unflatten(-1, (-1, 128))  # noqa: E731
+    held = lambda v, a: (blocks(v.abs()).sum(-1) * blocks(a).amax(-1)).sum(-1)  # noqa: E731  (sum of |v| of a block times its largest |a|)
+    for t in range(T):
+        want, bound = 0.0, 0.0
+        for j, e in enumerate(ids[t].tolist()):
+            xd, p = x[t].double(), probs[t, j].double()
+            u = v1[e] @ xd
+            du = (v1[e].abs() @ xd.abs() * 31 + s1[e] @ xd.abs() * (30 * 12)) * 2.0**-23 + held(v1[e], xd.abs()) * 2.0**-22
+            a, b = u[:I], u[I:]
+            h = a * torch.sigmoid(a) * b
+            # silu's slope is at most 1.1; between the products h is held to 2^-12 of itself or 2^-22 of the block's largest (a half-block's in
+            # larger batches), and silu and the products are within 8 roundings
+            dh = 1.1 * du[:I] * (b.abs() + du[I:]) + (a * torch.sigmoid(a)).abs() * du[I:] + h.abs() * (2.0**-12 + 8 * 2.0**-23)
+            dy = v2[e].abs() @ (dh + h.abs() * 91 * 2.0**-23) + (s2[e] @ h.abs()) * (30 * 12 * 2.0**-23) + held(v2[e], h.abs()) * 2.0**-22
+            want, bound = want + p * (v2[e] @ h), bound + p * dy
+        off, bound = (y[t] - want).abs(), bound + want.abs() * eps + torch.finfo(dtype).smallest_normal
+        assert bool((off <= bound).all()), (off / bound).max()
 
 
 # ---- the host side ----------------------------------------------------------------------------------------------------------------

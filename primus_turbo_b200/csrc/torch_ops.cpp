@@ -794,6 +794,7 @@ bool int4_parts(const Tensor &q, const Tensor &s, const std::optional<Tensor> &z
     auto fits = [&](const Tensor &t, ScalarType dt) { return bare(t) && t.is_contiguous() && t.device() == beside.device() && t.scalar_type() == dt; };
     if (group != 32 && group != 64 && group != 128) return false;
     if (!fits(q, ScalarType::Byte) || !aligned(q) || !fits(s, ScalarType::BFloat16) || (z && !fits(*z, ScalarType::Byte))) return false;
+    if (wants_grad(s) || has_tangent(s)) return false;
     return q.size(-1) == cdiv(k, 128) * 64 && s.size(-1) == cdiv(k, group) && (!z || z->sizes() == s.sizes());
 }
 const void *data_or_null(const std::optional<Tensor> &t) { return t ? t->const_data_ptr() : nullptr; }
@@ -873,7 +874,7 @@ py::object py_moe_few_tokens(const Tensor &x, const Tensor &ids, const Tensor &p
             if (w.size(2) != width || !w.is_contiguous() || !aligned(w) || w.device() != x.device()) return false;
             return format == code_of(x.scalar_type()) ? !s.has_value()
                                                      : is_fp8(w.scalar_type()) && s && bare(*s) && s->is_contiguous() && s->device() == x.device() &&
-                                                           s->scalar_type() == ScalarType::Float;
+                                                           s->scalar_type() == ScalarType::Float && !wants_grad(*s) && !has_tangent(*s);
         };
         if (!fits(w1, H, s1) || !fits(w2, inter, s2)) return py::none();
     }

@@ -1,6 +1,6 @@
 """4-bit weights with group scales: ``quantize_int4``, ``dequantize_int4`` and ``gemm_int4``, the product of a few rows of
 activations with one.  For serving: a weight is quantised once, when a model is loaded, and each token then reads a quarter of
-the bytes.  None of the three has a gradient; a call that would need one is refused.
+the bytes.  None of the three has a gradient; a call that would need one, of the activations or of the scales, is refused.
 
 The reference has no 4-bit integer format; names and argument order follow its FP8 ops (ops/quantization.py:52-269,
 ops/gemm_fp8.py:658 there).
@@ -67,6 +67,7 @@ def dequantize_int4(w: Int4Weight, out_dtype: torch.dtype = torch.bfloat16) -> t
         out = _native.ext.dequant_int4(w.qdata, w.scale, w.zero, w.shape[-1], w.group_size, out_dtype)
         if out is not None:
             return out
+    refuse_gradient("dequantize_int4", w.scale)
     require_cuda(w.qdata)
     return _ops.dequant_int4(w.qdata, w.scale, w.zero, w.shape[-1], w.group_size, out_dtype)
 
@@ -84,7 +85,7 @@ def gemm_int4(x: torch.Tensor, w: Int4Weight, bias: Optional[torch.Tensor] = Non
         y = _native.ext.gemm_int4(x, w.qdata, w.scale, w.zero, w.shape[-1], w.group_size, bias)
         if y is not None:
             return y
-    refuse_gradient("gemm_int4", x, bias)
+    refuse_gradient("gemm_int4", x, bias, w.scale)
     if w.ndim != 2:
         raise ValueError(f"gemm_int4 takes a 2D weight, got {w.ndim}D")
     if x.dtype not in (torch.bfloat16, torch.float16):

@@ -112,6 +112,7 @@ def moe_few_tokens(
     step = 16 if kind == "fp8" else 8
     if H < 1 or inter < 1 or H % step or inter % step:
         raise ValueError(f"the hidden and intermediate widths must be multiples of {step}, got {H} and {inter}")
+    refuse_gradient("moe_few_tokens", s1, s2)
     require_cuda(x, topk_ids, topk_probs, d1, d2)
     if any(t is not None and t.device != x.device for t in (topk_ids, topk_probs, d1, s1, z1, d2, s2, z2)):
         raise PtbError("moe_few_tokens: all tensors must be on one device")

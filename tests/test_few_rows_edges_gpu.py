@@ -158,6 +158,22 @@ def test_two_threads_launch_one_kernel_with_different_sizes():
     assert all(torch.equal(a, b) for o, w in zip(out, want) for a, b in zip(o, w))
 
 
+def test_scales_that_want_a_gradient_are_refused():
+    q = weight((16, 64), 64, False)
+    learned = Int4Weight(q.qdata, q.scale.clone().requires_grad_(), None, q.shape, 64)
+    x = torch.randn(3, 64, device=DEV, dtype=BF)
+    layer = [weight(s, 64, False) for s in ((2, 64, 64), (2, 64, 32))]
+    grown = [Int4Weight(w.qdata, w.scale.clone().requires_grad_(), None, w.shape, 64) for w in layer]
+    ids, probs = torch.zeros(3, 1, dtype=torch.int64, device=DEV), torch.ones(3, 1, device=DEV)
+    for call, same in ((lambda: gemm_int4(x, learned), lambda: gemm_int4(x, q)), (lambda: dequantize_int4(learned), lambda: dequantize_int4(q)),
+                       (lambda: moe_few_tokens(x, ids, probs, grown[0], layer[1]), lambda: moe_few_tokens(x, ids, probs, *layer)),
+                       (lambda: moe_few_tokens(x, ids, probs, layer[0], grown[1]), lambda: moe_few_tokens(x, ids, probs, *layer))):
+        with pytest.raises(NotImplementedError, match="no backward"):
+            call()
+        with torch.no_grad():
+            assert torch.equal(call(), same())
+
+
 def test_traced_quantising_runs_again_on_new_inputs():
     w, x, other = quantize_int4(torch.randn(72, 256, device=DEV, dtype=BF), 128), *(torch.randn(3, 256, device=DEV, dtype=BF) for _ in range(2))
     for f in (lambda x: x @ dequantize_int4(w).T, lambda x: quantize_int4(x, 32).qdata, lambda x: dequantize_int4(quantize_int4(x, 32, False))):

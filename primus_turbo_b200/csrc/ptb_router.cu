@@ -338,10 +338,12 @@ __global__ void __launch_bounds__(kRows * 32, V <= 8 ? 40 / kRows : 4) router_ke
             choose<uint32_t, V>(key, a.k, lane, first, my_e);
         }
     } else {
-        // 32-bit scores, fast and nearly right.  Of w, the largest score and bias: the fast exp is within 2 + 1.2 |x| units of its last
-        // place, which leaves at most 2^-21 w of error in a score; a softmax divides them all by one sum, off by (V + 5) 2^-24 w at the
-        // most; adding the bias 2^-24 w; the low bits that are given away V 2^-23 w.  Two scores further apart than the sum of
-        // these for both, below 2^-18 w + V 2^-22 w, are in their right order.
+        // 32-bit scores, fast and nearly right.  Of w, the largest score and bias, in units u = 2^-23 w: the fast exp is within 2 + 1.2 |x| units of
+        // its last place.  Softmax: exp(x) (2 + 1.7 |x|), x <= 0 (itself rounded), is largest at 0, so a score is off by 2 u, the sum that divides
+        // all alike left aside, and 1 for the product.  Sigmoid, s = 1 / (1 + exp(-x)): s ((2 + 1.2 |x|) (1 - s) + 2.5) is below 5 u where the
+        // largest logit is 0 or more (w is 1/2 at least), and below (5 + 1.2 |x|) u with x the largest logit where it is less, since s is about
+        // exp(x) and w may be no more.  Adding the bias 1/2 u; the low bits that are given away V u.  So two scores further apart than
+        // 11 u + 2 V u + 2.4 |x| u are in their right order: tol is more.  Below exp(-64) the quotient comes near its smallest numbers.
         float c[V], b[V], widest = 0.0f;
         load_bias<V>(a, first, b);
         float z = 0.0f;
@@ -359,8 +361,9 @@ __global__ void __launch_bounds__(kRows * 32, V <= 8 ? 40 / kRows : 4) router_ke
             key[j]        = l[j] == -INFINITY ? 0u : Places<V>::with(key_of(s + b[j]), j);
         }
         sort_down<V>(key);
-        const float tol = warp_max(widest) * (0x1p-18f + V * 0x1p-22f);
-        bool clear = tol < INFINITY;
+        const float below = a.softmax || top >= 0.0f || top == -INFINITY ? 0.0f : -top; // (of a row of nothing no score is compared)
+        const float tol   = warp_max(widest) * (0x1p-18f + V * 0x1p-22f + below * 0x1p-21f);
+        bool clear = tol < INFINITY && below <= 64.0f;
         if (a.groups > a.topk_groups) clear = keep_groups_sorted<V>(key, a, lane, first, 2.0f * tol) && clear;
         clear = choose_sorted<V, true>(key, a.k, lane, first, my_e, tol) && clear;
         if (!clear) my_e = choose_wide<T, V>(row, a, lane, vec); // (one answer for the warp)

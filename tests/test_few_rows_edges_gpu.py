@@ -1,6 +1,7 @@
 """GPU: inputs at the edges of what the few-row operators take: activations beside an outlier, infinite weights, logits far below
 zero, two host threads at once, the gradient's graph kept, traced quantising."""
 
+import math
 import threading
 
 import pytest
@@ -9,7 +10,7 @@ import torch
 from primus_turbo_b200 import _lib
 from primus_turbo_b200.pytorch.core.int4_weight import Int4Weight
 from primus_turbo_b200.pytorch.ops import dequantize_int4, gemm_int4, quantize_int4
-from primus_turbo_b200.pytorch.ops.moe import moe_few_tokens
+from primus_turbo_b200.pytorch.ops.moe import moe_few_tokens, topk_router
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -123,6 +124,30 @@ def test_a_layer_beside_an_outlier(T, dtype, where):
             want, bound = want + p * (v2[e] @ h), bound + p * dy
         off, bound = (y[t] - want).abs(), bound + want.abs() * eps + torch.finfo(dtype).smallest_normal
         assert bool((off <= bound).all()), (off / bound).max()
+
+
+# ---- router: rows of very negative logits -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("E", [4, 16, 64])
+@pytest.mark.parametrize("base", [-12.0, -33.0, -46.0, -62.0, -80.0, -86.0, -95.0])
+@pytest.mark.parametrize("bias", [False, True])
+def test_close_sigmoid_scores_far_below_zero(E, base, bias):
+    """Two groups of two whose logits are units of the last place away and add up to the same: what counts are the sums of the 64-bit scores."""
+    g = torch.Generator(DEV).manual_seed(E)
+    T, size = 1 << 18, E // 2
+    i, j = (torch.randint(0, 2048, (T,), device=DEV, generator=g) for _ in range(2))
+    d = torch.randint(1, 32, (T,), device=DEV, generator=g)
+    unit = 2.0 ** (math.floor(math.log2(-base)) - 23)
+    l = torch.full((T, E), 2 * base, device=DEV, dtype=torch.float64)
+    for e, v in ((0, i), (size - 1, j), (size, i + d), (E - 1, j - d)):
+        l[:, e] = base + v * unit
+    l = l.float()
+    s = 1 / (1 + torch.exp(-l.double()))
+    best = s.view(T, 2, size).sort(dim=2, descending=True).values[:, :, :2].sum(2)
+    other = (best[:, 1] > best[:, 0])[:, None].expand(T, E).clone()
+    other[:, size:] = ~other[:, size:]
+    want = s.masked_fill(other, -1.0).sort(dim=1, descending=True, stable=True).indices[:, :2]
+    _, ids = topk_router(l, 2, score_function="sigmoid", expert_bias=torch.zeros(E, device=DEV) if bias else None, num_groups=2, topk_groups=1)
+    assert torch.equal(ids, want), (ids != want).any(1).sum()
 
 
 # ---- the host side ----------------------------------------------------------------------------------------------------------------

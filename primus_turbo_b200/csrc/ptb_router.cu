@@ -533,7 +533,7 @@ int check_shape(const char *who, int64_t T, int64_t E, int64_t row_stride, int64
     PTB_REQUIRE(T >= 0 && E >= 1 && k >= 1 && k <= E, PTB_ERR_ARG, "%s: bad sizes", who);
     PTB_REQUIRE(E <= kMaxExperts, PTB_ERR_TOO_LARGE, "%s: more than %d experts", who, kMaxExperts);
     PTB_REQUIRE(k <= kMaxTopk, PTB_ERR_TOO_LARGE, "%s: more than %d experts per token", who, kMaxTopk);
-    PTB_REQUIRE(T <= 8ll * 2147483647ll, PTB_ERR_TOO_LARGE, "%s: too many tokens", who);
+    PTB_REQUIRE(T <= kRows * 2147483647ll, PTB_ERR_TOO_LARGE, "%s: too many tokens", who);
     PTB_REQUIRE(T <= 1 || row_stride >= E, PTB_ERR_ARG, "%s: rows overlap", who);
     PTB_REQUIRE(score_function == PTB_SCORE_SOFTMAX || score_function == PTB_SCORE_SIGMOID, PTB_ERR_ARG, "%s: unknown score function %d", who, score_function);
     return 0;

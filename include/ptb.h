@@ -491,7 +491,7 @@ int ptb_gemm_int4(const void *x, int dtype, int64_t ldx, int64_t M, int64_t N, i
  * [0, E) contributes nothing.  out [T, H] in x's type, contiguous.  x goes with 16-bit weights as it is,
  * otherwise held to 2^-22 of the largest finite value of its 128 channels or better.  Sums are kept in fp32, the activation between the two products
  * in fp16 scaled per 64 or 128 channels, with 16-bit weights or fp16 results in two parts, or as integers to 2^-22 of the largest of its 128 (4-bit
- * weights, few tokens); equal inputs give equal bits.
+ * weights, few tokens); equal inputs give equal bits.  An infinite weight or scale makes the results that it takes part in infinite or NaN.
  * format: x's own type code, PTB_E4M3, PTB_E5M2 or PTB_INT4, the same for both weights.  Data contiguous, 16-byte aligned.
  *   FP8: scale holds fp32 inverse scales, by granularity: PTB_TENSORWISE one, PTB_ROWWISE [E, rows], PTB_BLOCKWISE
  *        [E, ceil(rows / 128), ceil(K / 128)].  H and I multiples of 16.

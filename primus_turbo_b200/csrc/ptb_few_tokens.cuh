@@ -340,7 +340,7 @@ __device__ __forceinline__ void few_tokens_walk(uint8_t *smem, const CUtensorMap
                 bool there = token[j] < cols;
                 if constexpr (kMasked) there = there && src.mask(seg, token[j]);
                 if constexpr (FMT == kW16) {
-                    if (there)
+                    if (there && place[j] == 0) // (the other columns hold zeros, or, where a weight is infinite, NaN)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) acc[2 * h + j] += c[0][2 * h + j] + c[1][2 * h + j];
                 } else if (there && place[j] < filled) {

@@ -82,7 +82,8 @@ def moe_few_tokens(
 
     Activations are not quantised: with FP8 and 4-bit weights they are held to 2^-22 of the largest of their 128 neighbours or better
     (what is above 2^-11 of it is exact), with 16-bit weights as they are.  Sums are kept in fp32, and the activation between the two
-    products in more than bf16; the result is rounded once to x's type.  Equal inputs give equal bits.  Every call allocates its own workspace, so calls on
+    products in more than bf16; the result is rounded once to x's type.  What an infinite weight or scale takes part in is infinite or NaN.
+    Equal inputs give equal bits.  Every call allocates its own workspace, so calls on
     several streams or in several captured graphs do not share any."""
     if _native.usable(x):
         y = _native_layer(x, topk_ids, topk_probs, w_gate_up, w_down)

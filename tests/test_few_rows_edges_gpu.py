@@ -9,6 +9,8 @@ import torch
 
 from primus_turbo_b200 import _lib
 from primus_turbo_b200.pytorch.core.int4_weight import Int4Weight
+from primus_turbo_b200.pytorch.core.low_precision import Float8QuantConfig, ScalingGranularity
+from primus_turbo_b200.pytorch.core.quantized_tensor import create_quantized_weight
 from primus_turbo_b200.pytorch.ops import dequantize_int4, gemm_int4, quantize_int4
 from primus_turbo_b200.pytorch.ops.moe import moe_few_tokens, topk_router
 
@@ -124,6 +126,62 @@ def test_a_layer_beside_an_outlier(T, dtype, where):
             want, bound = want + p * (v2[e] @ h), bound + p * dy
         off, bound = (y[t] - want).abs(), bound + want.abs() * eps + torch.finfo(dtype).smallest_normal
         assert bool((off <= bound).all()), (off / bound).max()
+
+
+# ---- infinite weights -----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 5, 8, 9, 20])
+@pytest.mark.parametrize("dtype", [BF, torch.float16])
+def test_an_infinite_weight_of_16_bits_is_infinite_in_any_batch(T, dtype):
+    """An infinity in the up projection: in bf16 the same signed infinities whatever the number of tokens, and nothing where it takes no part.
+    In fp16 the down projection's weights are the sum of two bf16, of either sign: an infinity times one less an infinity times the other is NaN."""
+    E, H, I = 3, 256, 128
+    g = torch.Generator(DEV).manual_seed(T)
+    w1, w2 = (torch.randn(E, 2 * I, H, device=DEV, generator=g) / 16).to(dtype), (torch.randn(E, H, I, device=DEV, generator=g) / 11).to(dtype)
+    w1[1, I + 3, 40] = math.inf
+    w1[1, 3] = w1[1, 3].abs()  # its gate is positive for positive x
+    x = (torch.rand(T, H, device=DEV, generator=g) + 0.5).to(dtype)
+    ids = (torch.arange(T, device=DEV) % 3)[:, None].flip(0).contiguous()
+    if T == 1:
+        ids[0] = 1
+    y = moe_few_tokens(x, ids, torch.ones(T, 1, device=DEV), w1, w2)
+    sign = torch.sign(w2[1, :, 3].double())
+    for t in range(T):
+        if ids[t, 0] == 1:
+            if dtype == BF:
+                assert torch.equal(y[t].double()[sign != 0], (sign * math.inf)[sign != 0])
+            else:
+                assert not y[t].isfinite().any()
+        else:
+            assert bool(y[t].isfinite().all())
+
+
+@pytest.mark.parametrize("kind", ["raw", "e5m2", "int4"])
+@pytest.mark.parametrize("T", [1, 2, 3, 8, 9])
+def test_an_infinite_weight_shows_where_it_takes_part(kind, T):
+    """In the down projection: infinite or NaN in its output column for the tokens of its expert, nothing else touched."""
+    E, H, I = 4, 256, 256
+    g = torch.Generator(DEV).manual_seed(T)
+    w1, w2 = (torch.randn(E, 2 * I, H, device=DEV, generator=g) / 16).to(BF), (torch.randn(E, H, I, device=DEV, generator=g) / 16).to(BF)
+    if kind == "int4":
+        w1, w2 = quantize_int4(w1, 64), quantize_int4(w2, 64)
+    elif kind == "e5m2":
+        cfg = Float8QuantConfig(granularity=ScalingGranularity.BLOCKWISE, block_size=128)
+        w1, w2 = (create_quantized_weight(w, torch.float8_e5m2, cfg)[0] for w in (w1, w2))
+    x = torch.randn(T, H, device=DEV, generator=g).to(BF)
+    ids = torch.rand(T, E, device=DEV, generator=g).argsort(1)[:, :2].contiguous()
+    ids[0, 0], ids[0, 1] = 1, 2
+    probs = torch.rand(T, 2, device=DEV, generator=g) + 0.1
+    before = moe_few_tokens(x, ids, probs, w1, w2)
+    if kind == "int4":
+        w2.scale[1, 77, 3] = math.inf
+    elif kind == "e5m2":
+        w2.qdata.view(torch.uint8)[1, 77, 200] = 0x7C
+    else:
+        w2[1, 77, 200] = math.inf
+    y = moe_few_tokens(x, ids, probs, w1, w2)
+    hit = torch.zeros(T, H, dtype=torch.bool, device=DEV)
+    hit[:, 77] = (ids == 1).any(1)
+    assert not y[hit].isfinite().any() and torch.equal(y[~hit], before[~hit])
 
 
 # ---- router: rows of very negative logits -----------------------------------------------------------------------------------------

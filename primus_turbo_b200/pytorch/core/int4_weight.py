@@ -21,6 +21,11 @@ def _packed_bytes(k: int) -> int:
     return (k + INT4_BLOCK - 1) // INT4_BLOCK * INT4_BLOCK_BYTES
 
 
+def _has_values(t: torch.Tensor) -> bool:
+    """Not a stand-in of a tensor, as while tracing."""
+    return not (t.is_meta or torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0)
+
+
 @dataclass(frozen=True)
 class Int4Weight:
     """``[N, K]`` or ``[E, N, K]``; made by ``quantize_int4`` or ``from_codes``."""
@@ -68,10 +73,19 @@ class Int4Weight:
     def from_codes(
         cls, codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor] = None, *, group_size: int
     ) -> "Int4Weight":
-        """From codes 0 .. 15, one a byte, ``[..., N, K]``; ``scale`` and ``zero`` ``[..., N, ceil(K / group_size)]``."""
+        """From codes 0 .. 15, one a byte, ``[..., N, K]``; ``scale`` and ``zero`` ``[..., N, ceil(K / group_size)]``.
+
+        Scales are kept in bfloat16.  Others are taken where bfloat16 holds every one of them exactly; where it does not, rounding them
+        (``scale.to(torch.bfloat16)``, up to 2^-8 of each weight) is left to the caller.  For these checks the codes and such scales are read
+        back: this is for loading a model, not for a captured graph."""
         assert codes.dtype == torch.uint8, "codes must be uint8, one code (0 .. 15) a byte"
         k = codes.shape[-1]
         assert k % 8 == 0, f"the row length of a 4-bit weight must be a multiple of 8, got {k}"
+        if _has_values(codes) and codes.numel() > 0:
+            assert int(codes.max()) <= 15, f"codes must be 0 .. 15, got {int(codes.max())}"
+        if scale.dtype != torch.bfloat16 and _has_values(scale):
+            kept = (scale.to(torch.bfloat16).to(scale.dtype) == scale) | scale.isnan()
+            assert bool(kept.all()), f"these {scale.dtype} scales are not bfloat16 numbers: pass scale.to(torch.bfloat16) to have them rounded"
         padded = torch.nn.functional.pad(codes, (0, -k % INT4_BLOCK)) if k % INT4_BLOCK else codes
         octets = padded.unflatten(-1, (-1, 4, 4, 8)).transpose(-2, -3)  # [..., block, t, q, 8]
         qdata = (octets[..., :4] & 15 | octets[..., 4:] << 4).flatten(-4).contiguous()

@@ -46,3 +46,29 @@ def test_scales_with_a_tangent_are_refused():
         for call in calls(lambda shape: fwAD.make_dual(torch.ones(shape, dtype=BF), torch.ones(shape, dtype=BF))):
             with pytest.raises(NotImplementedError, match="forward mode"):
                 call()
+
+
+# ---- from_codes takes what it can hold -----------------------------------------------------------------------------------------
+def test_from_codes_refuses_scales_that_would_be_rounded():
+    codes = torch.randint(0, 16, (4, 64), dtype=torch.uint8)
+    for dtype in (torch.float16, torch.float32, torch.float64):
+        held = torch.tensor([[0.5], [1.0078125], [float("nan")], [float("inf")]], dtype=dtype)
+        assert torch.equal(Int4Weight.from_codes(codes, held, group_size=64).scale.double().nan_to_num(7.0), held.double().nan_to_num(7.0))
+        for bad in (1.0009765625, 65504.0, 0.1):
+            scale = held.clone()
+            scale[1, 0] = bad
+            with pytest.raises(AssertionError, match="bfloat16"):
+                Int4Weight.from_codes(codes, scale, group_size=64)
+            rounded = scale.to(BF)
+            assert torch.equal(Int4Weight.from_codes(codes, rounded, group_size=64).scale[:2], rounded[:2])
+
+
+def test_from_codes_refuses_codes_of_more_than_four_bits():
+    codes = torch.zeros(2, 3, 64, dtype=torch.uint8)
+    scale = torch.ones(2, 3, 1, dtype=BF)
+    Int4Weight.from_codes(codes, scale, group_size=64)
+    codes[1, 2, 63] = 16
+    with pytest.raises(AssertionError, match="15"):
+        Int4Weight.from_codes(codes, scale, group_size=64)
+    assert Int4Weight.from_codes(codes[:0], scale[:0], group_size=64).shape == (0, 3, 64)
+    assert Int4Weight.from_codes(codes.to("meta"), scale.to("meta"), group_size=64).shape == (2, 3, 64)

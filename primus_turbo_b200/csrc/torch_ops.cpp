@@ -19,6 +19,8 @@
 #include <pybind11/pybind11.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <atomic>
@@ -923,7 +925,6 @@ struct RouterFn : public torch::autograd::Function<RouterFn> {
         return {probs, chosen};
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
-        TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), "the gradient of topk_router has no derivative of its own (create_graph)");
         return in_backward([&] {
             const auto sv = ctx->get_saved_variables();
             const Tensor &l = sv[0], &ids = sv[1];
@@ -935,6 +936,10 @@ struct RouterFn : public torch::autograd::Function<RouterFn> {
             PTB_RUN(ptb_topk_router_bwd, l.const_data_ptr(), code_of(l.scalar_type()), l.size(0), l.size(1), l.stride(0), ids.size(1), (int) (spec & 255),
                     (int) (spec >> 8 & 1), (float) ctx->saved_data["scaling"].toDouble(), ids.const_data_ptr<int64_t>(), g.const_data_ptr<float>(), g.stride(0),
                     (int) (spec >> 9 & 1), out.mutable_data_ptr(), c.st);
+            if (at::GradMode::is_enabled()) // create_graph: whoever differentiates the gradient, by the logits too, is told that it has no derivative
+                torch::autograd::set_history(out, std::make_shared<torch::autograd::Error>(
+                                                      "trying to differentiate topk_router twice: its gradient has no derivative",
+                                                      torch::autograd::collect_next_edges(l)));
             return variable_list{out, Tensor(), Tensor()};
         });
     }

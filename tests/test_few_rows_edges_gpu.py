@@ -241,6 +241,19 @@ def test_two_threads_launch_one_kernel_with_different_sizes():
     assert all(torch.equal(a, b) for o, w in zip(out, want) for a, b in zip(o, w))
 
 
+def test_create_graph_is_taken_and_its_derivative_refused():
+    logits = torch.randn(5, 16, device=DEV, requires_grad=True)
+    probs, _ = topk_router(logits, 3)
+    (want,) = torch.autograd.grad(probs.square().sum(), logits)
+    probs, _ = topk_router(logits, 3)
+    (g,) = torch.autograd.grad(probs.square().sum(), logits, create_graph=True)
+    assert torch.equal(g, want)
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(g.sum(), logits, retain_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(probs.sum() + g.norm(), logits)
+
+
 def test_scales_that_want_a_gradient_are_refused():
     q = weight((16, 64), 64, False)
     learned = Int4Weight(q.qdata, q.scale.clone().requires_grad_(), None, q.shape, 64)

@@ -10,7 +10,6 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from primus_turbo_b200 import _native
 from primus_turbo_b200._lib import PtbError, require_cuda
@@ -20,6 +19,18 @@ from primus_turbo_b200.pytorch.kernels.few_rows_impl import SCORE_FUNCTIONS
 __all__ = ["topk_router", "topk_routing_map"]
 
 _MAX_EXPERTS, _MAX_TOPK, _MAX_GROUPS = 1024, 32, 32
+
+
+class _NoSecondDerivative(torch.autograd.Function):
+    """The gradient itself, kept in the graph (create_graph) as a function of the logits whose derivative is refused."""
+
+    @staticmethod
+    def forward(ctx, dl, logits):
+        return dl.view_as(dl)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("trying to differentiate topk_router twice: its gradient has no derivative")
 
 
 class _TopkRouter(torch.autograd.Function):
@@ -33,10 +44,13 @@ class _TopkRouter(torch.autograd.Function):
         return probs, chosen
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad, _):
         logits, ids = ctx.saved_tensors
-        return (_ops.topk_router_bwd(logits, ids, grad, *ctx.options),) + (None,) * 8
+        with torch.no_grad():
+            dl = _ops.topk_router_bwd(logits, ids, grad, *ctx.options)
+        if torch.is_grad_enabled() and not torch.compiler.is_compiling():
+            dl = _NoSecondDerivative.apply(dl, logits)
+        return (dl,) + (None,) * 8
 
 
 def _route(logits, topk, score_function, expert_bias, num_groups, topk_groups, normalize, scaling_factor, dense):

@@ -7,7 +7,7 @@ import threading
 import pytest
 import torch
 
-from primus_turbo_b200 import _lib
+from primus_turbo_b200 import _lib, _native
 from primus_turbo_b200.pytorch.core.int4_weight import Int4Weight
 from primus_turbo_b200.pytorch.core.low_precision import Float8QuantConfig, ScalingGranularity
 from primus_turbo_b200.pytorch.core.quantized_tensor import create_quantized_weight
@@ -241,7 +241,10 @@ def test_two_threads_launch_one_kernel_with_different_sizes():
     assert all(torch.equal(a, b) for o, w in zip(out, want) for a, b in zip(o, w))
 
 
-def test_create_graph_is_taken_and_its_derivative_refused():
+@pytest.mark.parametrize("native", [True, False])
+def test_create_graph_is_taken_and_its_derivative_refused(monkeypatch, native):
+    if not native:
+        monkeypatch.setattr(_native, "usable", lambda t: False)
     logits = torch.randn(5, 16, device=DEV, requires_grad=True)
     probs, _ = topk_router(logits, 3)
     (want,) = torch.autograd.grad(probs.square().sum(), logits)

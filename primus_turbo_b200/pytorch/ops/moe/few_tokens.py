@@ -79,6 +79,8 @@ def moe_few_tokens(
     1024 (an id outside [0, E) contributes nothing: padding, or a token with too few experts); ``w_gate_up`` [E, 2 I, H]
     with the gate rows first and ``w_down`` [E, H, I], both plain tensors of x's type, both FP8 ``QuantizedTensor`` (tensorwise, rowwise
     or 128 x 128 blockwise scales, of one kind), or both ``Int4Weight`` of one group size.  H and I are multiples of 8, of 16 for FP8.
+    Weights are read where they lie if they are contiguous and start on 16 bytes; a plain tensor that is not (a transposed view of
+    another layout) is copied whole in every call, so lay such a weight out once.
 
     Activations are not quantised: with FP8 and 4-bit weights they are held to 2^-22 of the largest of their 128 neighbours or better
     (what is above 2^-11 of it is exact), with 16-bit weights as they are.  Sums are kept in fp32, and the activation between the two

@@ -498,7 +498,7 @@ int ptb_gemm_int4(const void *x, int dtype, int64_t ldx, int64_t M, int64_t N, i
  *   4-bit: the layout of ptb_quant_int4 for E * rows rows; zero may be NULL; one group size for both.  H, I multiples of 8.
  * T <= PTB_MOE_FEW_MAX_TOKENS, T * k <= PTB_MOE_FEW_MAX_PAIRS, E <= 1024.  workspace: 16-byte aligned, of
  * ptb_moe_few_tokens_workspace bytes (-1: sizes out of range); calls that may overlap need one each.
- * For more tokens the grouped GEMMs above are the way.  No counterpart in the reference. */
+ * For more tokens the grouped GEMMs above are the way (after ptb_dequant_int4 for 4-bit weights).  No counterpart in the reference. */
 #define PTB_INT4 5
 #define PTB_MOE_FEW_MAX_TOKENS 128
 #define PTB_MOE_FEW_MAX_PAIRS 1024

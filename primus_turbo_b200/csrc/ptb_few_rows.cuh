@@ -3,8 +3,8 @@
 //
 // Such a product reads the weight once and does little with it, so it is bound by HBM, and everything here serves to have
 // many wide loads in flight and few instructions per weight.  The weight takes the 16-row side of mma.sync and eight rows of x the
-// other: tcgen05 wants 128 weight rows and its operands in shared memory, unpacked, which at one to sixteen rows buys nothing but a copy.  A
-// warp walks 128-wide blocks of k; its weights come as tensor boxes into two slots of its own, which it fills again as soon as it has
+// other: tcgen05 wants 128 weight rows, unpacked, in shared or tensor memory, which at one to sixteen rows buys nothing but a copy (for more it may pay; it
+// has not been built).  A warp walks 128-wide blocks of k; its weights come as tensor boxes into two slots of its own, which it fills again as soon as it has
 // read them.  No barrier of the CTA stands in the walk.
 //
 // What an MMA is fed with.  Measured on a B200, an SM issues an m16n8k16 of 16-bit floats or an m16n8k32 of bytes every 2.1 clocks (FP8
@@ -13,11 +13,11 @@
 //   * for a token or a few (few_tokens_walk) 4-bit codes go in as the bytes they are: two ANDs and a shift for 8 codes.  x is an integer
 //     of three bytes, the first signed, scaled by a power of two per block that brings the largest of its 128 to 2^21 .. 2^22.  bf16's eight bits are
 //     exact in it down to 2^-14 of the largest, fp16's eleven to 2^-11; below, a value is off by up to 2^-22 of the largest.  (With two bytes 2^-15: beside
-//     an outlier of 1000 the result of the others is off by more than bf16's own rounding.  The third costs 5 %: 4096 x 14336, one row, 11.3 instead of
-//     10.7 us, and room: rows that no longer fit are for the other walk, 2 rows of 14336 19.5 instead of 13.5.)  Sums of
+//     an outlier of 1000 the result of the others is off by more than bf16's own rounding.  The third costs 3 %: 4096 x 14336, one row, 12.1 instead of
+//     11.7 us, and room: rows that no longer fit are for the other walk, 2 rows of 14336 19.5 instead of 13.5.)  Sums of
 //     a group are exact integers, and scaling them is what costs: with more columns of x than eight it is too much;
 //   * for more (few_rows_walk) codes become fp16 less their zero, exactly, 9 instructions for 8.  That is what bounds it: 48 tokens through 32
-//     experts of 7168 x 2048, groups of 32, 351 us where the weights' 790 MB are 121, with two thirds of all issue slots used.  Of these, scaling
+//     experts of 7168 x 2048, groups of 32, 357 us where the weights' 790 MB are 121, with two thirds of all issue slots used.  Of these, scaling
 //     the sums of the groups and their MMAs are a fifth, unpacking an eighth, fetching scales a tenth;
 //   * FP8 weights are converted to fp16, exactly, one instruction for two;
 //   * x goes with fp16 weights as fp16, scaled by a power of two per block into its range, where bf16 and fp16 values are exact down

@@ -10,17 +10,18 @@
 //  * moe_down_token_kernel: a tile is 16 output columns of all experts, whose blocks of k are one long k; the eight columns of the
 //    MMA are the tokens.  Nothing is added in memory: no atomics, no second pass, and the same bits every time.
 //
-// Measured: 8 of 128 experts of 2048 x 768 in 4 bits 13 us, 8 experts of 7168 x 2048 in FP8 63 us, where the weights are 54.
+// Measured: 8 of 128 experts of 2048 x 768 in 4 bits 15 us (the weights are 3), 8 experts of 7168 x 2048 in FP8 62 us, where the weights are 54.
 //
 // For more tokens four: moe_list_kernel sorts the pairs by expert, beside the scaling of x; moe_gate_up_kernel on an expert's own tokens;
 // moe_down_kernel writes a 32-bit row per pair and moe_merge_kernel adds up a token's rows in the router's order.
 //
-// Measured: FP8, 24 tokens, 128 experts of 2048 x 768, 89 us where the weights that are hit are 73; 4-bit see ptb_few_rows.cuh; 16-bit, 64 tokens, 16
-// experts of 2880 x 1440, 122 us where the weights are 61: its 368 CTAs have 296 places, and the second wave leaves three quarters of them empty.
+// Measured: FP8, 24 tokens, 128 experts of 2048 x 768, 93 us where the weights that are hit are 73; 4-bit see ptb_few_rows.cuh; 16-bit, 64 tokens, 16
+// experts of 2880 x 1440, 106 us where the weights are 61: its 368 CTAs have 296 places, and the second wave leaves three quarters of them empty.
 //
 // The activation h between the two products is kept in 32 bits and then scaled like x, or scaled at once, per 64 channels: to fp16
 // (2^-12 of each value; with fp16 results what that leaves is a second term), for 4-bit weights and few tokens to integers (2^-22 of the
-// block's largest).  With 16-bit weights it is two bf16 (2^-17).  Its rounding is not felt in the result.
+// block's largest).  With 16-bit weights it is two bf16 (2^-17).  One fp16 turns over the
+// last bit of some bf16 results (8e-4 of their norm, where rounding them is 1.7e-3); the other forms are hardly felt.
 #include "ptb_few_tokens.cuh"
 
 namespace ptb {

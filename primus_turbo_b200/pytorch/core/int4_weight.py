@@ -23,7 +23,8 @@ def _packed_bytes(k: int) -> int:
 
 def _has_values(t: torch.Tensor) -> bool:
     """Not a stand-in of a tensor, as while tracing."""
-    return not (t.is_meta or torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0)
+    plain = type(t) in (torch.Tensor, torch.nn.Parameter) and not t.is_meta
+    return plain and not torch.compiler.is_compiling() and torch._C._len_torch_dispatch_stack() == 0
 
 
 @dataclass(frozen=True)

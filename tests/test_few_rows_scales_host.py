@@ -72,3 +72,11 @@ def test_from_codes_refuses_codes_of_more_than_four_bits():
         Int4Weight.from_codes(codes, scale, group_size=64)
     assert Int4Weight.from_codes(codes[:0], scale[:0], group_size=64).shape == (0, 3, 64)
     assert Int4Weight.from_codes(codes.to("meta"), scale.to("meta"), group_size=64).shape == (2, 3, 64)
+
+
+def test_from_codes_of_stand_ins():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        codes, scale = torch.empty(4, 64, dtype=torch.uint8), torch.empty(4, 1, dtype=torch.float16)
+        assert Int4Weight.from_codes(codes, scale, group_size=64).scale.dtype == BF
